@@ -559,7 +559,22 @@ int nkv_transfer_synchronize(nkv_transfer* lane);
  *                whose count reaches zero goes to the back of the queue;
  *     APPEND     slot takes one block from the queue front (the reference
  *                calls may_append when len(seq) % block_size == 1);
- *     FENCE      no-op.
+ *     FENCE      no-op;
+ *     FORK       slot (empty) becomes a copy of another sequence's first
+ *                num_blocks blocks: args at args_offset = [parent slot,
+ *                pair index].  Each is held once more; with a pair index
+ *                >= 0 the last one, partly filled, is replaced by a fresh
+ *                block from the queue front and copies[pair index] =
+ *                {the parent's block, the fresh one} (-1: shared too);
+ *     COMPACT    args at args_offset = [first pair index].  Of U blocks in
+ *                use, the k-th at or past U moves to the k-th free one
+ *                below it: tables and counts follow, the free queue becomes
+ *                U, U + 1, ..., copies[first + k] = {old, new} and the
+ *                number of moves goes to meta[5].
+ *   Neither has a counterpart in the reference.  Both need
+ *   nkv_pool_apply_copies, whose `copies` holds max_copies int32 pairs; the
+ *   pages themselves are moved by nkv_copy_blocks.  A FORK's pair is only
+ *   good until a later op frees its source.
  *   Consecutive APPENDs, and consecutive ALLOCATEs without cached ids, run
  *   as one parallel step up to the first repeated slot; the result is the
  *   one-op-at-a-time result.
@@ -569,7 +584,7 @@ int nkv_transfer_synchronize(nkv_transfer* lane);
  *   ends the log; later logs are ignored until nkv_pool_init.
  * The arrays (at nkv_pool_offsets[k], in the order of the NKV_POOL_* ids):
  *     META   int64[8] = head, tail, live free blocks, error op + 1, error
- *            code;
+ *            code, moves of the last COMPACT;
  *     RING   int32[2*num_blocks], the queue, -1 tombstones;
  *     QPOS   int64[num_blocks];
  *     REF    int32[num_blocks];
@@ -591,6 +606,8 @@ typedef struct nkv_pool_desc {
 #define NKV_POOL_OP_DEALLOCATE 2
 #define NKV_POOL_OP_APPEND 3
 #define NKV_POOL_OP_FENCE 4
+#define NKV_POOL_OP_FORK 5
+#define NKV_POOL_OP_COMPACT 6
 #define NKV_POOL_META 0
 #define NKV_POOL_RING 1
 #define NKV_POOL_QPOS 2
@@ -613,6 +630,9 @@ int nkv_pool_offsets(int64_t num_blocks, int64_t max_seqs,
 int nkv_pool_init(const nkv_pool_desc* pool, void* stream);
 int nkv_pool_apply(const nkv_pool_desc* pool, const int32_t* ops, int64_t num_ops,
                    const int32_t* args, int64_t num_args, void* stream);
+int nkv_pool_apply_copies(const nkv_pool_desc* pool, const int32_t* ops,
+                          int64_t num_ops, const int32_t* args, int64_t num_args,
+                          int32_t* copies, int64_t max_copies, void* stream);
 int nkv_pack_decode_pool(const nkv_pool_desc* pool, const int32_t* num_tokens,
                          const int32_t* seq_slots, int64_t num_seqs,
                          int64_t padded_seqs, int64_t block_size,
@@ -629,6 +649,67 @@ int nkv_pack_prefill_pool(const nkv_pool_desc* pool, const int32_t* num_cached,
                           int32_t* block_tables, int32_t* full_context_lens,
                           int32_t* query_start_lens, int32_t* max_seqlens,
                           void* stream);
+
+/*
+ * Pages copied: page pairs[i][0] of src to page pairs[i][1] of dst in every
+ * plane, planes being the [num_blocks, block] caches laid end to end in the
+ * two allocations (K and V of every layer: 2 * layers).  src and dst may be
+ * one allocation; no destination may be named twice, nor be a source of
+ * another pair (its page would hold either's bytes).  Pairs with an id
+ * outside [0, src_blocks) x [0, dst_blocks) are skipped.  Bits are moved; a
+ * page has block_bytes bytes (even).  No counterpart in the reference.
+ */
+int nkv_copy_blocks(const void* src, void* dst, int64_t planes,
+                    int64_t src_blocks, int64_t dst_blocks, int64_t block_bytes,
+                    const int32_t* pairs, int64_t num_pairs, void* stream);
+
+/*
+ * Rotary positions.  No counterpart in the paged path of the reference: its
+ * attention is given rotated heads (nanovllm/layers/attention.py:75-93).
+ * nkv_rotary_table fills table[max_position][rotary_dim / 2] float2 with
+ *   (factor cos a, factor sin a), a = position * inv_freq[j],
+ * computed in fp64 from the rotary_dim / 2 device doubles inv_freq.
+ * nkv_rotary turns pair j of the first rotary_dim dims of every query and key
+ * head, dims (j, j + rotary_dim / 2) (NKV_ROTARY_HALF) or (2 j, 2 j + 1)
+ * (NKV_ROTARY_INTERLEAVED), by the table's row of its token's position:
+ *   (x1 cos - x2 sin, x2 cos + x1 sin), fp32, rounded once;
+ * other dims are copied.  positions holds num_tokens int32 or int64, or three
+ * rows of them position_row_stride apart (0: one row): pairs [0, ends[0])
+ * take the first row, [ends[0], ends[1]) the second, the rest the third.
+ * Queries go to q_out, keys to k_out (may be NULL when they are stored);
+ * either may be its own input (same pointer and strides).  With key_cache
+ * and value_cache the rotated keys and the values also go to their slots as
+ * nkv_store puts them (-1 and slots outside the cache: not stored).  A token
+ * with a position outside [0, max_position) gets zero outputs and is not
+ * stored.  Strides in elements; the dims of a head are contiguous.
+ */
+#define NKV_ROTARY_HALF 0
+#define NKV_ROTARY_INTERLEAVED 1
+#define NKV_ROTARY_MAX_HEAD_DIM 1024
+#define NKV_ROTARY_MAX_HEADS 1024
+typedef struct nkv_rotary_desc {
+  const void* q;               /* [num_tokens, num_q_heads, head_dim] */
+  const void* k;               /* [num_tokens, num_kv_heads, head_dim] */
+  const void* v;               /* as k; only read with the caches */
+  void* q_out;
+  void* k_out;
+  void* key_cache;             /* [num_slots, num_kv_heads, head_dim] or NULL */
+  void* value_cache;
+  const void* positions;
+  const int32_t* slot_mapping; /* [num_tokens]; only read with the caches */
+  const float* table;          /* 16-byte aligned */
+  int64_t num_tokens, num_q_heads, num_kv_heads, head_dim, rotary_dim;
+  int64_t max_position, num_slots;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride;
+  int64_t v_token_stride, v_head_stride;
+  int64_t q_out_token_stride, q_out_head_stride;
+  int64_t k_out_token_stride, k_out_head_stride;
+  int64_t position_row_stride, section_ends[2];
+  int32_t position_bytes, layout, dtype, reserved;
+} nkv_rotary_desc;
+int nkv_rotary_table(const double* inv_freq, double factor, int64_t max_position,
+                     int64_t rotary_dim, float* table, void* stream);
+int nkv_rotary(const nkv_rotary_desc* desc, void* stream);
 
 #ifdef __cplusplus
 }

@@ -30,6 +30,12 @@
 // anything; the first invalid op is recorded in meta and ends the log, so
 // the state is always the reference's state after the valid prefix of the
 // log.
+//
+// Two ops have no counterpart there.  FORK gives an empty slot the first
+// blocks of another sequence, each held once more, with a fresh block from
+// the queue front in the place of a partly filled last one; COMPACT moves
+// the blocks in use to the low ids.  Both list the pages to copy as
+// {source, destination} pairs (nkv_copy_blocks moves them).
 #include "nkv_common.h"
 
 namespace nkv {
@@ -223,11 +229,74 @@ __device__ int32_t run_length(const PoolView& v, const int4* __restrict__ ops, i
   return cut;
 }
 
-// ops: int4 per op {type, slot, num_blocks (allocate), args offset
-// (allocate)}; args[off] = number of cached ids, args[off+1 ...] the ids.
+// COMPACT: of U blocks in use, the k-th at or past U moves to the k-th free
+// one below it.  Tables, counts and the free queue (ids U, U + 1, ... in
+// order) follow; the moves go to copies[first ...] and their number to
+// meta[5].  Each thread ranks a run of consecutive ids, so the ranks cost two
+// scans whatever the pool's size; the ring and qpos, which are rewritten at
+// the end, hold the holes and the new names meanwhile.
+// Returns false, with nothing changed, where the moves do not fit.
+__device__ bool compact_blocks(const PoolView& v, Cursor& c, int2* __restrict__ copies, int64_t first,
+                               int64_t max_copies, int32_t* s_tmp) {
+  const int32_t t = threadIdx.x;
+  const int32_t used = v.num_blocks - static_cast<int32_t>(c.live);
+  const int32_t per = (v.num_blocks + kPoolThreads - 1) / kPoolThreads;
+  const int32_t begin = static_cast<int32_t>(min<int64_t>(v.num_blocks, static_cast<int64_t>(t) * per));
+  const int32_t end = static_cast<int32_t>(min<int64_t>(v.num_blocks, static_cast<int64_t>(begin) + per));
+  int32_t holes = 0, movers = 0;
+  for (int32_t b = begin; b < end; ++b) {
+    if (b < used) {
+      holes += v.ref[b] == 0 ? 1 : 0;
+    } else {
+      movers += v.ref[b] > 0 ? 1 : 0;
+    }
+  }
+  int32_t total = 0, moves = 0;
+  int32_t hole = block_exclusive_scan<kPoolThreads>(holes, s_tmp, &total);
+  int32_t mover = block_exclusive_scan<kPoolThreads>(movers, s_tmp, &moves);
+  if (moves != total || first < 0 || first + moves > max_copies) return false;
+  for (int32_t b = begin; b < min(end, used); ++b) {
+    if (v.ref[b] == 0) v.ring[hole++] = b;
+  }
+  __syncthreads();
+  for (int32_t b = max(begin, used); b < end; ++b) {
+    if (v.ref[b] > 0) {
+      const int32_t to = v.ring[mover];
+      copies[first + mover] = make_int2(b, to);
+      ++mover;
+      v.ref[to] = v.ref[b];
+      v.ref[b] = 0;
+      v.qpos[b] = to;
+    }
+  }
+  __syncthreads();
+  const int64_t cells = static_cast<int64_t>(v.max_seqs) * v.width;
+  for (int64_t i = t; i < cells; i += kPoolThreads) {
+    const int32_t b = v.tables[i];
+    if (b >= used && b < v.num_blocks) v.tables[i] = static_cast<int32_t>(v.qpos[b]);
+  }
+  __syncthreads();
+  for (int64_t i = t; i < v.cap; i += kPoolThreads) {
+    v.ring[i] = i < v.num_blocks - used ? used + static_cast<int32_t>(i) : -1;
+  }
+  for (int32_t b = t; b < v.num_blocks; b += kPoolThreads) v.qpos[b] = b < used ? -1 : b - used;
+  if (t == 0) v.meta[5] = moves;
+  c.head = 0;
+  c.tail = v.num_blocks - used;
+  c.live = v.num_blocks - used;
+  __syncthreads();
+  return true;
+}
+
+// ops: int4 per op {type, slot, num_blocks (allocate, fork), args offset
+// (allocate, fork, compact)}; args[off] = number of cached ids, args[off+1
+// ...] the ids (allocate); the parent slot, then the index of the pair to
+// write or -1 when the last block is shared too (fork); the index of the
+// first pair (compact).
 __global__ __launch_bounds__(kPoolThreads) void pool_apply_kernel(
     PoolView v, const int4* __restrict__ ops, int64_t num_ops,
-    const int32_t* __restrict__ args, int64_t num_args) {
+    const int32_t* __restrict__ args, int64_t num_args, int2* __restrict__ copies,
+    int64_t max_copies) {
   __shared__ int32_t s_tmp[kPoolThreads / kWave + 1];
   __shared__ int32_t s_pre[kPoolThreads + 1];
   __shared__ int32_t s_slot[kPoolThreads];
@@ -408,6 +477,131 @@ __global__ __launch_bounds__(kPoolThreads) void pool_apply_kernel(
         i += run;
         continue;
       }
+    }
+
+    if (op.x == NKV_POOL_OP_FORK) {
+      // A run of forks into distinct slots, none of them from a slot that an
+      // earlier op of the run fills: validated first, then one parallel pop
+      // for the copied last blocks and one pass over the shared ones.
+      int4 mine;
+      int32_t run = run_length(
+          v, ops, i, num_ops,
+          [&](const int4& o) { return o.x == NKV_POOL_OP_FORK && o.w >= 0 && o.w + 1 < num_args; },
+          &s_end, &mine);
+      if (run == 0) {
+        err = kErrBadArgs;
+        err_op = i;
+        break;
+      }
+      const int32_t parent = t < run ? args[mine.w] : -1;
+      const int32_t pair = t < run ? args[mine.w + 1] : -1;
+      const bool slot_ok = t < run && mine.y >= 0 && mine.y < v.max_seqs;
+      const bool parent_ok = t < run && parent >= 0 && parent < v.max_seqs;
+      // Slot marks name the op of the run that fills a slot.
+      if (slot_ok) v.slot_mark[mine.y] = t + 1;
+      if (t == 0) s_end = run;
+      __syncthreads();
+      if (parent_ok) {
+        const int32_t by = v.slot_mark[parent];
+        if (by > 0 && by - 1 < t) atomicMin(&s_end, t);
+      }
+      __syncthreads();
+      if (slot_ok) v.slot_mark[mine.y] = 0;
+      run = s_end;
+      __syncthreads();
+      if (t == 0) s_bad = run;
+      __syncthreads();
+      int32_t code = 0;
+      if (t < run) {
+        if (!slot_ok || !parent_ok || parent == mine.y) {
+          code = kErrBadSlot;
+        } else if (v.nblk[mine.y] != 0) {
+          code = kErrTableBusy;
+        } else if (mine.z < 0 || mine.z > v.width || mine.z > v.nblk[parent] || pair < -1 ||
+                   pair >= max_copies || (pair >= 0 && mine.z == 0)) {
+          code = kErrBadArgs;
+        }
+        if (code != 0) atomicMin(&s_bad, t);
+      }
+      __syncthreads();
+      // The parents' blocks of the ops before the first bad one.
+      int32_t cells = 0;
+      const int32_t mine_cells = t < s_bad ? mine.z : 0;
+      const int32_t cell0 = block_exclusive_scan<kPoolThreads>(mine_cells, s_tmp, &cells);
+      const int32_t runs = s_bad;  // ops whose cells are counted
+      if (t < runs) {
+        s_pre[t] = cell0;
+        s_slot[t] = parent;
+      }
+      if (t == 0) s_pre[runs] = cells;
+      __syncthreads();
+      for (int32_t x = t; x < cells; x += kPoolThreads) {
+        const int32_t k = owner_of(s_pre, runs, x);
+        const int32_t b = v.tables[static_cast<int64_t>(s_slot[k]) * v.width + (x - s_pre[k])];
+        if (b < 0 || b >= v.num_blocks || v.ref[b] <= 0) atomicMin(&s_bad, k);
+      }
+      __syncthreads();
+      if (t < run && code == 0 && t == s_bad) code = kErrBadBlock;
+      const int32_t first_bad = s_bad;
+      __syncthreads();
+      if (t == first_bad && first_bad < run) s_bad = code;  // broadcast its code
+      __syncthreads();
+      const int32_t bad_code = first_bad < run ? s_bad : 0;
+      // Fresh blocks, one per copied last block; the first op without one.
+      int32_t fresh = 0;
+      const int32_t takes = t < first_bad && pair >= 0 ? 1 : 0;
+      const int32_t before = block_exclusive_scan<kPoolThreads>(takes, s_tmp, &fresh);
+      if (t == 0) s_end = first_bad;
+      __syncthreads();
+      if (takes && before + 1 > c.live) atomicMin(&s_end, t);
+      __syncthreads();
+      const int32_t ok = s_end;
+      const int32_t pops = static_cast<int32_t>(min<int64_t>(fresh, c.live));
+      // The shared blocks of the valid ops: held once more each.
+      const int32_t valid_cells = ok > 0 ? s_pre[ok] : 0;
+      for (int32_t x = t; x < valid_cells; x += kPoolThreads) {
+        const int32_t k = owner_of(s_pre, ok, x);
+        const int4 o = ops[i + k];
+        const int32_t j = x - s_pre[k];
+        if (j == o.z - 1 && args[o.w + 1] >= 0) continue;  // copied, below
+        const int32_t b = v.tables[static_cast<int64_t>(s_slot[k]) * v.width + j];
+        v.tables[static_cast<int64_t>(o.y) * v.width + j] = b;
+        atomicAdd(&v.ref[b], 1);
+      }
+      __syncthreads();
+      if (takes && t < ok) s_slot[before] = t;  // the op of the pop numbered `before`
+      __syncthreads();
+      pop_front(v, c, pops, s_tmp, &s_pos, [&](int32_t k, int32_t b) {
+        const int4 o = ops[i + s_slot[k]];
+        const int32_t from = args[o.w];
+        const int32_t last = v.tables[static_cast<int64_t>(from) * v.width + o.z - 1];
+        v.tables[static_cast<int64_t>(o.y) * v.width + o.z - 1] = b;
+        v.ref[b] = 1;
+        copies[args[o.w + 1]] = make_int2(last, b);
+      });
+      if (t < ok) v.nblk[mine.y] = mine.z;
+      // The counts were raised in L2: later plain reads must not find older
+      // ones in this CU's cache.
+      __threadfence();
+      __syncthreads();
+      if (ok < run) {
+        err = ok == first_bad ? bad_code : kErrNoFreeBlocks;
+        err_op = i + ok;
+        break;
+      }
+      i += run;
+      continue;
+    }
+
+    if (op.x == NKV_POOL_OP_COMPACT) {
+      if (op.w < 0 || op.w >= num_args ||
+          !compact_blocks(v, c, copies, args[op.w], max_copies, s_tmp)) {
+        err = kErrBadArgs;
+        err_op = i;
+        break;
+      }
+      ++i;
+      continue;
     }
 
     const int32_t slot = op.y;
@@ -592,8 +786,19 @@ extern "C" int nkv_pool_init(const nkv_pool_desc* pool, void* stream) {
 
 extern "C" int nkv_pool_apply(const nkv_pool_desc* pool, const int32_t* ops, int64_t num_ops,
                               const int32_t* args, int64_t num_args, void* stream) {
+  return nkv_pool_apply_copies(pool, ops, num_ops, args, num_args, nullptr, 0, stream);
+}
+
+extern "C" int nkv_pool_apply_copies(const nkv_pool_desc* pool, const int32_t* ops, int64_t num_ops,
+                                     const int32_t* args, int64_t num_args, int32_t* copies,
+                                     int64_t max_copies, void* stream) {
   using namespace nkv;
   if (int rc = check_desc(pool, "nkv_pool_apply")) return rc;
+  if (max_copies < 0 || max_copies > INT32_MAX || (max_copies > 0 && copies == nullptr) ||
+      reinterpret_cast<uint64_t>(copies) % 8 != 0) {
+    return nkv_fail(NKV_E_INVALID,
+                    "nkv_pool_apply: copies must be 8-byte aligned and hold max_copies in [0, 2^31) pairs");
+  }
   if (num_ops < 0 || num_args < 0 || num_ops > INT32_MAX || num_args > INT32_MAX) {
     return nkv_fail(NKV_E_INVALID, "nkv_pool_apply: negative or oversized op log");
   }
@@ -605,7 +810,8 @@ extern "C" int nkv_pool_apply(const nkv_pool_desc* pool, const int32_t* ops, int
     return nkv_fail(NKV_E_INVALID, "nkv_pool_apply: ops must be 16-byte aligned");
   }
   pool_apply_kernel<<<dim3(1), dim3(kPoolThreads), 0, static_cast<hipStream_t>(stream)>>>(
-      view_of(*pool), reinterpret_cast<const int4*>(ops), num_ops, args, num_args);
+      view_of(*pool), reinterpret_cast<const int4*>(ops), num_ops, args, num_args,
+      reinterpret_cast<int2*>(copies), max_copies);
   return nkv_check_launch("nkv_pool_apply");
 }
 

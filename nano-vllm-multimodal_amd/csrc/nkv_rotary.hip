@@ -1,0 +1,345 @@
+// Rotary positions: the query and key heads of a layer turned by the angles
+// of their tokens' positions, on their own or on the way into the paged
+// cache (the keys rotated and stored, the values stored, one launch).
+//
+// Pair j of a head's first rotary_dim dims, (x1, x2) = dims (j, j +
+// rotary_dim / 2) in the half layout or (2 j, 2 j + 1) in the interleaved
+// one, becomes
+//   (x1 cos a - x2 sin a, x2 cos a + x1 sin a),  a = position * inv_freq[j],
+// in fp32 with one rounding to the element type; the other dims pass
+// through.  The angles of far positions need more than fp32 (position 131071
+// at one radian per position has an fp32 spacing of 2^-7), so cosine and
+// sine come from a table built once in fp64, [max_position][rotary_dim / 2]
+// float2; a factor of the scaling multiplies both.
+#include "nkv_common.h"
+
+namespace nkv {
+namespace {
+
+__global__ __launch_bounds__(256) void rotary_table_kernel(const double* __restrict__ inv_freq,
+                                                           double factor, int64_t entries,
+                                                           int32_t half, float2* __restrict__ table) {
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; e < entries; e += stride) {
+    const int64_t position = e / half;
+    double sine, cosine;
+    sincos(static_cast<double>(position) * inv_freq[e - position * half], &sine, &cosine);
+    table[e] = make_float2(static_cast<float>(cosine * factor), static_cast<float>(sine * factor));
+  }
+}
+
+// Element types: to and from fp32 (rounded to nearest even).
+struct Bf16 {
+  typedef uint16_t T;
+  static __device__ __forceinline__ float get(T v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
+  static __device__ __forceinline__ T put(float f) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f)); }
+};
+struct Fp16 {
+  typedef uint16_t T;
+  static __device__ __forceinline__ float get(T v) { return static_cast<float>(__builtin_bit_cast(_Float16, v)); }
+  static __device__ __forceinline__ T put(float f) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)); }
+};
+struct Fp32 {
+  typedef float T;
+  static __device__ __forceinline__ float get(T v) { return v; }
+  static __device__ __forceinline__ T put(float f) { return f; }
+};
+
+// One launch: strides in elements.  A null k_out, or key_cache, is not written.
+struct RotaryArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_out;
+  void* key_cache;
+  void* value_cache;
+  const void* positions;
+  const int32_t* slots;
+  const float2* table;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  int64_t q_out_token, q_out_head, k_out_token, k_out_head;
+  int64_t position_row;  // elements between position rows (sections), 0 without
+  int64_t max_position, num_slots;
+  int32_t num_tokens, q_heads, kv_heads, head_dim, half, wide_positions;
+  int32_t section_end0, section_end1;  // first pairs of the second and third position row
+  int32_t heads_apart;                 // heads a thread's steps are apart
+  int32_t token_threads;               // threads per token
+};
+
+// A thread handles two W-element vectors of a head: dims [W i, W i + W) and
+// the same past half (half layout), or 2 W dims in a row (interleaved): in
+// both the pairs [W i, W i + W), whose angles it loads once and keeps for
+// every head_apart-th head of its token.  Past the rotated dims its vectors
+// pass through.
+template <typename E, int W, bool kInterleaved, bool kStore>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
+  typedef typename E::T T;
+  typedef T Vec __attribute__((ext_vector_type(W)));
+  struct alignas(sizeof(T) * W) Pack {
+    T e[W];
+  };
+  const int64_t thread = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int32_t token = static_cast<int32_t>(thread / a.token_threads);
+  if (token >= a.num_tokens) return;
+  const int32_t rest = static_cast<int32_t>(thread - static_cast<int64_t>(token) * a.token_threads);
+  const int32_t lanes = (a.head_dim + 2 * W - 1) / (2 * W);  // threads of a head
+  const int32_t h0 = rest / lanes;
+  const int32_t lane = rest - h0 * lanes;
+  const int32_t j0 = lane * W;  // first pair, when rotated
+  const bool rotated = j0 < a.half;
+  const int32_t at1 = kInterleaved || !rotated ? 2 * j0 : j0;
+  const int32_t at2 = kInterleaved || !rotated ? 2 * j0 + W : j0 + a.half;
+  const bool both = at2 < a.head_dim;  // (an odd dim at the end, W == 1)
+
+  // The token's position of pair j.
+  auto position_of = [&](int32_t j) -> int64_t {
+    const int64_t row = a.position_row == 0 || j < a.section_end0 ? 0 : j < a.section_end1 ? 1 : 2;
+    const int64_t at = row * a.position_row + token;
+    return a.wide_positions ? static_cast<const int64_t*>(a.positions)[at]
+                            : static_cast<const int32_t*>(a.positions)[at];
+  };
+  float cosine[W], sine[W];
+  bool known = true;  // every position of the token is in the table
+  {
+    const int32_t rows = a.position_row == 0 ? 1 : 3;
+    for (int32_t r = 0; r < rows; ++r) {
+      const int64_t p = a.wide_positions
+                            ? static_cast<const int64_t*>(a.positions)[r * a.position_row + token]
+                            : static_cast<const int32_t*>(a.positions)[r * a.position_row + token];
+      known = known && p >= 0 && p < a.max_position;
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    cosine[w] = 1.f;
+    sine[w] = 0.f;
+  }
+  if (rotated && known) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float2 cs = a.table[position_of(j0 + w) * a.half + j0 + w];
+      cosine[w] = cs.x;
+      sine[w] = cs.y;
+    }
+  }
+  int64_t slot = -1;
+  if (kStore) {
+    slot = a.slots[token];
+    if (slot >= a.num_slots || !known) slot = -1;
+  }
+
+  const int32_t heads = a.q_heads + (kStore ? 2 : 1) * a.kv_heads;
+  for (int32_t h = h0; h < heads; h += a.heads_apart) {
+    const bool is_q = h < a.q_heads;
+    const int32_t kh = h - a.q_heads;
+    const bool is_v = kStore && kh >= a.kv_heads;
+    if (is_v) {
+      if (slot < 0) continue;
+      const int32_t vh = kh - a.kv_heads;
+      const T* src = static_cast<const T*>(a.v) + token * a.v_token + vh * a.v_head;
+      T* dst = static_cast<T*>(a.value_cache) + (slot * a.kv_heads + vh) * a.head_dim;
+      *reinterpret_cast<Pack*>(dst + 2 * j0) = *reinterpret_cast<const Pack*>(src + 2 * j0);
+      if (2 * j0 + W < a.head_dim) {
+        *reinterpret_cast<Pack*>(dst + 2 * j0 + W) = *reinterpret_cast<const Pack*>(src + 2 * j0 + W);
+      }
+      continue;
+    }
+    const T* src = is_q ? static_cast<const T*>(a.q) + token * a.q_token + h * a.q_head
+                        : static_cast<const T*>(a.k) + token * a.k_token + kh * a.k_head;
+    Pack x = *reinterpret_cast<const Pack*>(src + at1), y{};
+    if (both) y = *reinterpret_cast<const Pack*>(src + at2);
+    if (!known) {
+      x = Pack{};
+      y = Pack{};
+    } else if (rotated) {
+      float f[2 * W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        f[w] = E::get(x.e[w]);
+        f[W + w] = E::get(y.e[w]);
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const int i1 = kInterleaved ? 2 * w : w, i2 = kInterleaved ? 2 * w + 1 : W + w;
+        const float x1 = f[i1], x2 = f[i2];
+        f[i1] = x1 * cosine[w] - x2 * sine[w];
+        f[i2] = x2 * cosine[w] + x1 * sine[w];
+      }
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        x.e[w] = E::put(f[w]);
+        y.e[w] = E::put(f[W + w]);
+      }
+    }
+    if (is_q) {
+      T* dst = static_cast<T*>(a.q_out) + token * a.q_out_token + h * a.q_out_head;
+      *reinterpret_cast<Pack*>(dst + at1) = x;
+      if (both) *reinterpret_cast<Pack*>(dst + at2) = y;
+      continue;
+    }
+    if (a.k_out != nullptr) {
+      T* dst = static_cast<T*>(a.k_out) + token * a.k_out_token + kh * a.k_out_head;
+      *reinterpret_cast<Pack*>(dst + at1) = x;
+      if (both) *reinterpret_cast<Pack*>(dst + at2) = y;
+    }
+    if (kStore && slot >= 0) {
+      T* dst = static_cast<T*>(a.key_cache) + (slot * a.kv_heads + kh) * a.head_dim;
+      *reinterpret_cast<Pack*>(dst + at1) = x;
+      if (both) *reinterpret_cast<Pack*>(dst + at2) = y;
+    }
+  }
+}
+
+template <typename E, int W>
+void (*rotary_kernel_for(bool interleaved, bool store))(RotaryArgs) {
+  if (interleaved) return store ? rotary_kernel<E, W, true, true> : rotary_kernel<E, W, true, false>;
+  return store ? rotary_kernel<E, W, false, true> : rotary_kernel<E, W, false, false>;
+}
+
+}  // namespace
+}  // namespace nkv
+
+extern "C" int nkv_rotary_table(const double* inv_freq, double factor, int64_t max_position,
+                                int64_t rotary_dim, float* table, void* stream) {
+  using namespace nkv;
+  if (rotary_dim <= 0 || rotary_dim % 2 != 0 || rotary_dim > NKV_ROTARY_MAX_HEAD_DIM ||
+      max_position <= 0 || max_position > INT32_MAX) {
+    return nkv_fail(NKV_E_INVALID,
+                    "nkv_rotary_table: need an even rotary_dim in [2, %d] and max_position in [1, 2^31)",
+                    NKV_ROTARY_MAX_HEAD_DIM);
+  }
+  if (!inv_freq || !table) return nkv_fail(NKV_E_INVALID, "nkv_rotary_table: null pointer");
+  if (reinterpret_cast<uint64_t>(table) % 16 != 0) {
+    return nkv_fail(NKV_E_INVALID, "nkv_rotary_table: table must be 16-byte aligned");
+  }
+  const int64_t entries = max_position * (rotary_dim / 2);
+  const int64_t blocks = (entries + 255) / 256;
+  rotary_table_kernel<<<dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0,
+                        static_cast<hipStream_t>(stream)>>>(
+      inv_freq, factor, entries, static_cast<int32_t>(rotary_dim / 2), reinterpret_cast<float2*>(table));
+  return nkv_check_launch("nkv_rotary_table");
+}
+
+extern "C" int nkv_rotary(const nkv_rotary_desc* d, void* stream) {
+  using namespace nkv;
+  if (d == nullptr) return nkv_fail(NKV_E_INVALID, "nkv_rotary: null descriptor");
+  const int eb = element_bytes(d->dtype);
+  if (eb == 0) return nkv_fail(NKV_E_INVALID, "nkv_rotary: unknown dtype %d", d->dtype);
+  if (d->num_tokens < 0 || d->num_q_heads < 0 || d->num_kv_heads < 0 || d->head_dim <= 0 ||
+      d->head_dim > NKV_ROTARY_MAX_HEAD_DIM || d->num_q_heads > NKV_ROTARY_MAX_HEADS ||
+      d->num_kv_heads > NKV_ROTARY_MAX_HEADS || d->num_tokens > INT32_MAX) {
+    return nkv_fail(NKV_E_INVALID,
+                    "nkv_rotary: tokens outside [0, 2^31), heads outside [0, %d] or head_dim outside [1, %d]",
+                    NKV_ROTARY_MAX_HEADS, NKV_ROTARY_MAX_HEAD_DIM);
+  }
+  if (d->rotary_dim < 2 || d->rotary_dim % 2 != 0 || d->rotary_dim > d->head_dim) {
+    return nkv_fail(NKV_E_INVALID, "nkv_rotary: rotary_dim must be even, in [2, head_dim]");
+  }
+  if (d->layout != NKV_ROTARY_HALF && d->layout != NKV_ROTARY_INTERLEAVED) {
+    return nkv_fail(NKV_E_INVALID, "nkv_rotary: unknown layout %d", d->layout);
+  }
+  if (d->position_bytes != 4 && d->position_bytes != 8) {
+    return nkv_fail(NKV_E_INVALID, "nkv_rotary: positions must be 4 or 8 bytes each");
+  }
+  if (d->max_position <= 0 || d->max_position > INT32_MAX) {
+    return nkv_fail(NKV_E_INVALID, "nkv_rotary: max_position must be in [1, 2^31)");
+  }
+  const int64_t half = d->rotary_dim / 2;
+  if (d->position_row_stride < 0 ||
+      (d->position_row_stride > 0 &&
+       (d->section_ends[0] < 0 || d->section_ends[1] < d->section_ends[0] || d->section_ends[1] > half))) {
+    return nkv_fail(NKV_E_INVALID,
+                    "nkv_rotary: sections must split the pairs in order: 0 <= end0 <= end1 <= rotary_dim / 2");
+  }
+  const bool store = d->key_cache != nullptr || d->value_cache != nullptr;
+  if (d->num_slots < 0 || d->num_slots > INT32_MAX) {
+    return nkv_fail(NKV_E_INVALID, "nkv_rotary: num_slots outside [0, 2^31)");
+  }
+  for (int64_t s : {d->q_token_stride, d->q_head_stride, d->k_token_stride, d->k_head_stride,
+                    d->v_token_stride, d->v_head_stride, d->q_out_token_stride, d->q_out_head_stride,
+                    d->k_out_token_stride, d->k_out_head_stride}) {
+    if (s < 0) return nkv_fail(NKV_E_INVALID, "nkv_rotary: negative stride");
+  }
+  if (d->num_tokens == 0 || d->num_q_heads + d->num_kv_heads == 0) return NKV_OK;
+  if (!d->positions || !d->table || (d->num_q_heads > 0 && (!d->q || !d->q_out)) ||
+      (d->num_kv_heads > 0 && (!d->k || (!store && !d->k_out))) ||
+      (store && (!d->key_cache || !d->value_cache || !d->v || !d->slot_mapping))) {
+    return nkv_fail(NKV_E_INVALID, "nkv_rotary: null pointer");
+  }
+  // 16-byte vectors where every pointer, stride and part of a head allows
+  // them, single elements otherwise (head views cut at odd places).
+  const uint64_t vec = 16 / static_cast<uint64_t>(eb);
+  uint64_t bits = 0;
+  for (const void* p : {d->q, d->k, static_cast<const void*>(d->q_out), static_cast<const void*>(d->k_out),
+                        store ? d->v : nullptr, static_cast<const void*>(d->key_cache),
+                        static_cast<const void*>(d->value_cache)}) {
+    bits |= reinterpret_cast<uint64_t>(p);
+  }
+  if (bits % static_cast<uint64_t>(eb) != 0 || reinterpret_cast<uint64_t>(d->table) % 16 != 0 ||
+      reinterpret_cast<uint64_t>(d->positions) % static_cast<uint64_t>(d->position_bytes) != 0) {
+    return nkv_fail(NKV_E_INVALID, "nkv_rotary: pointers not aligned to their elements (table: 16 bytes)");
+  }
+  uint64_t strides = 0;
+  for (int64_t s : {d->q_token_stride, d->q_head_stride, d->k_token_stride, d->k_head_stride,
+                    d->q_out_token_stride, d->q_out_head_stride}) {
+    strides |= static_cast<uint64_t>(s);
+  }
+  if (store) strides |= static_cast<uint64_t>(d->v_token_stride) | static_cast<uint64_t>(d->v_head_stride);
+  if (d->k_out) strides |= static_cast<uint64_t>(d->k_out_token_stride) | static_cast<uint64_t>(d->k_out_head_stride);
+  const bool wide = bits % 16 == 0 && strides % vec == 0 && half % static_cast<int64_t>(vec) == 0 &&
+                    d->head_dim % static_cast<int64_t>(2 * vec) == 0;
+  const int64_t w = wide ? static_cast<int64_t>(vec) : 1;
+  const int64_t lanes = (d->head_dim + 2 * w - 1) / (2 * w);
+  const int64_t heads = d->num_q_heads + (store ? 2 : 1) * d->num_kv_heads;
+  int64_t apart = heads;
+  while (apart > 8 && d->num_tokens * lanes * apart > 256 * 2048) apart = (apart + 1) / 2;
+  const int64_t threads = lanes * apart;
+  const int64_t blocks = (d->num_tokens * threads + 255) / 256;
+  if (blocks > INT32_MAX) return nkv_fail(NKV_E_INVALID, "nkv_rotary: too many tokens for one launch");
+  RotaryArgs a{};
+  a.q = d->q;
+  a.k = d->k;
+  a.v = d->v;
+  a.q_out = d->q_out;
+  a.k_out = d->k_out;
+  a.key_cache = d->key_cache;
+  a.value_cache = d->value_cache;
+  a.positions = d->positions;
+  a.slots = d->slot_mapping;
+  a.table = reinterpret_cast<const float2*>(d->table);
+  a.q_token = d->q_token_stride;
+  a.q_head = d->q_head_stride;
+  a.k_token = d->k_token_stride;
+  a.k_head = d->k_head_stride;
+  a.v_token = d->v_token_stride;
+  a.v_head = d->v_head_stride;
+  a.q_out_token = d->q_out_token_stride;
+  a.q_out_head = d->q_out_head_stride;
+  a.k_out_token = d->k_out_token_stride;
+  a.k_out_head = d->k_out_head_stride;
+  a.position_row = d->position_row_stride;
+  a.max_position = d->max_position;
+  a.num_slots = d->num_slots;
+  a.num_tokens = static_cast<int32_t>(d->num_tokens);
+  a.q_heads = static_cast<int32_t>(d->num_q_heads);
+  a.kv_heads = static_cast<int32_t>(d->num_kv_heads);
+  a.head_dim = static_cast<int32_t>(d->head_dim);
+  a.half = static_cast<int32_t>(half);
+  a.wide_positions = d->position_bytes == 8 ? 1 : 0;
+  a.section_end0 = static_cast<int32_t>(d->section_ends[0]);
+  a.section_end1 = static_cast<int32_t>(d->section_ends[1]);
+  a.heads_apart = static_cast<int32_t>(apart);
+  a.token_threads = static_cast<int32_t>(threads);
+  const bool inter = d->layout == NKV_ROTARY_INTERLEAVED;
+  void (*kernel)(RotaryArgs) = nullptr;
+  if (d->dtype == NKV_DTYPE_FLOAT32) {
+    kernel = wide ? rotary_kernel_for<Fp32, 4>(inter, store) : rotary_kernel_for<Fp32, 1>(inter, store);
+  } else if (d->dtype == NKV_DTYPE_FLOAT16) {
+    kernel = wide ? rotary_kernel_for<Fp16, 8>(inter, store) : rotary_kernel_for<Fp16, 1>(inter, store);
+  } else {
+    kernel = wide ? rotary_kernel_for<Bf16, 8>(inter, store) : rotary_kernel_for<Bf16, 1>(inter, store);
+  }
+  kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(a);
+  return nkv_check_launch("nkv_rotary");
+}

@@ -45,6 +45,26 @@ class PoolDesc(ctypes.Structure):
 
 c_pool = ctypes.POINTER(PoolDesc)
 
+
+class RotaryDesc(ctypes.Structure):
+    """struct nkv_rotary_desc."""
+
+    _fields_ = [
+        *((name, ctypes.c_void_p) for name in (
+            "q", "k", "v", "q_out", "k_out", "key_cache", "value_cache", "positions",
+            "slot_mapping", "table")),
+        *((name, ctypes.c_int64) for name in (
+            "num_tokens", "num_q_heads", "num_kv_heads", "head_dim", "rotary_dim", "max_position",
+            "num_slots", "q_token_stride", "q_head_stride", "k_token_stride", "k_head_stride",
+            "v_token_stride", "v_head_stride", "q_out_token_stride", "q_out_head_stride",
+            "k_out_token_stride", "k_out_head_stride", "position_row_stride")),
+        ("section_ends", ctypes.c_int64 * 2),
+        *((name, ctypes.c_int32) for name in ("position_bytes", "layout", "dtype", "reserved")),
+    ]
+
+
+c_rotary = ctypes.POINTER(RotaryDesc)
+
 # name -> (restype, argtypes); mirrors include/nanokv.h.
 SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "nkv_version": (ctypes.c_int, ()),
@@ -166,6 +186,12 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "nkv_pool_offsets": (ctypes.c_int, (c_i64, c_i64, c_i64, c_i64_out)),
     "nkv_pool_init": (ctypes.c_int, (c_pool, c_ptr)),
     "nkv_pool_apply": (ctypes.c_int, (c_pool, c_ptr, c_i64, c_ptr, c_i64, c_ptr)),
+    "nkv_pool_apply_copies": (
+        ctypes.c_int, (c_pool, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr)),
+    "nkv_copy_blocks": (
+        ctypes.c_int, (c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr)),
+    "nkv_rotary_table": (ctypes.c_int, (c_ptr, ctypes.c_double, c_i64, c_i64, c_ptr, c_ptr)),
+    "nkv_rotary": (ctypes.c_int, (c_rotary, c_ptr)),
     "nkv_pack_decode_pool": (
         ctypes.c_int,
         (c_pool, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr,
@@ -182,6 +208,8 @@ NKV_POOL_OP_ALLOCATE = 1
 NKV_POOL_OP_DEALLOCATE = 2
 NKV_POOL_OP_APPEND = 3
 NKV_POOL_OP_FENCE = 4
+NKV_POOL_OP_FORK = 5
+NKV_POOL_OP_COMPACT = 6
 NKV_POOL_ERRORS = {
     1: "unknown op type",
     2: "slot outside [0, max_seqs)",
@@ -191,6 +219,9 @@ NKV_POOL_ERRORS = {
     6: "block id out of range or not owned",
     7: "bad counts or args offset",
 }
+
+NKV_ROTARY_HALF = 0
+NKV_ROTARY_INTERLEAVED = 1
 
 NKV_DTYPE_FLOAT16 = 0
 NKV_DTYPE_BFLOAT16 = 1

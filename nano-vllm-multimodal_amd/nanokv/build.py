@@ -30,6 +30,8 @@ SOURCES = (
     "nkv_pool.hip",
     "nkv_noalloc.hip",
     "nkv_store_gather.hip",
+    "nkv_rotary.hip",
+    "nkv_pages.hip",
 )
 OFFLOAD_ARCH = "gfx950"
 HIPCC_FLAGS = (

@@ -21,6 +21,7 @@ from nanokv import _lib
 from nanokv.paged_kv import ops
 from nanokv.paged_kv.base import (
     PagedKVAllocation,
+    index_value_validation_enabled,
     validate_store_inputs,
 )
 
@@ -451,6 +452,113 @@ class HIPPagedKVBackend:
         ops.paged_attention_prefill(q, key_cache, value_cache, block_tables, cu_seqlens_q,
                                     cu_seqlens_k, plan, float(softmax_scale), out)
         return out
+
+    # ------------------------------------------------- rotary positions
+    def rotary(
+        self,
+        q: torch.Tensor,
+        k: torch.Tensor,
+        positions: torch.Tensor,
+        table,
+        *,
+        out: tuple[torch.Tensor, torch.Tensor] | None = None,
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """q [T, Hq, D] and k [T, Hkv, D] (float16, bfloat16 or float32; views
+        of a fused projection as they are) turned by the angles of
+        ``positions`` ([T] int32 or int64, or [3, T] for a table with
+        sections), a :class:`nanokv.rotary.RotaryTable`.  ``out`` = (q_out,
+        k_out) may be the inputs themselves, or memory of its own.  A token
+        whose position is outside the table gets zeros."""
+        if not _READY:
+            self._load()
+        validate_positions(positions, table)
+        if out is None:
+            out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+                   torch.empty(k.shape, dtype=k.dtype, device=k.device))
+        ops.rotary(q, k, positions, table.table, table.layout_code, table.section_ends, out[0], out[1])
+        return out
+
+    def rotary_store(
+        self,
+        q: torch.Tensor,
+        k: torch.Tensor,
+        v: torch.Tensor,
+        key_cache: torch.Tensor,
+        value_cache: torch.Tensor,
+        slot_mapping: torch.Tensor,
+        positions: torch.Tensor,
+        table,
+        *,
+        q_out: torch.Tensor | None = None,
+        k_out: torch.Tensor | None = None,
+    ) -> torch.Tensor:
+        """:meth:`rotary` and the layer's :meth:`store` in one launch: the
+        rotated keys and the values go to their slots, the rotated queries
+        are returned (``q_out``, which may be q itself).  ``k_out`` also
+        receives the rotated keys, for attention over keys in place.  A
+        token whose position is outside the table gets zeros and is not
+        stored."""
+        if not _READY:
+            self._load()
+        validate_store_inputs(k, v, key_cache, value_cache, slot_mapping)
+        validate_positions(positions, table)
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ops.rotary_store(q, k, v, key_cache, value_cache, slot_mapping, positions, table.table,
+                         table.layout_code, table.section_ends, q_out, k_out)
+        return q_out
+
+    # ------------------------------------------------------------- pages
+    def copy_blocks(
+        self,
+        cache: torch.Tensor,
+        pairs: torch.Tensor | Sequence[tuple[int, int]],
+        *,
+        dst: torch.Tensor | None = None,
+    ) -> None:
+        """Blocks pairs[i][0] of ``cache`` [.., blocks, block, kv_heads,
+        head_dim] copied to blocks pairs[i][1], in every plane (the leading
+        dims: K and V of every layer) by one launch; with ``dst`` into
+        another cache, which may have another number of blocks.
+
+        No destination may be named twice or be another pair's source.
+        Pairs from the host are checked; pairs on the device ([n, 2] int32,
+        as DeviceBlockPool gives them) only when index validation is on:
+        ids outside the caches are skipped there, and a block named against
+        that rule ends with bytes of either."""
+        if not _READY:
+            self._load()
+        target = cache if dst is None else dst
+        if not isinstance(pairs, torch.Tensor):
+            pairs = torch.tensor([tuple(p) for p in pairs], dtype=torch.int32).reshape(-1, 2)
+        if pairs.ndim != 2 or pairs.shape[1] != 2 or pairs.dtype not in (torch.int32, torch.int64):
+            raise ValueError("block copy: pairs must be [n, 2] int32")
+        if cache.ndim < 4 or target.ndim < 4:
+            raise ValueError("block copy requires [.., blocks, block, kv_heads, head_dim] caches")
+        if pairs.shape[0] and index_value_validation_enabled(pairs):
+            validate_block_pairs(pairs, cache.shape[-4], target.shape[-4],
+                                 same=target.data_ptr() == cache.data_ptr())
+        if not pairs.is_cuda:
+            pairs = pairs.to(device=cache.device, dtype=torch.int32)
+        ops.copy_blocks(cache, target, pairs)
+
+
+def validate_positions(positions: torch.Tensor, table) -> None:
+    """Position values, when index validation is enabled (it synchronises)."""
+    if positions.numel() and index_value_validation_enabled(positions):
+        if bool(((positions < 0) | (positions >= table.max_position)).any()):
+            raise ValueError(f"positions contain one outside [0, {table.max_position})")
+
+
+def validate_block_pairs(pairs: torch.Tensor, src_blocks: int, dst_blocks: int, *, same: bool) -> None:
+    """The rules of copy_blocks on pair values."""
+    source, to = pairs.cpu().long().unbind(1)
+    if bool(((source < 0) | (source >= src_blocks) | (to < 0) | (to >= dst_blocks)).any()):
+        raise ValueError("block copy: a pair names a block outside the cache")
+    if torch.unique(to).numel() != to.numel():
+        raise ValueError("block copy: a destination is named twice")
+    if same and bool(torch.isin(to[source != to], source).any()):
+        raise ValueError("block copy: a destination is another pair's source")
 
 
 def validate_varlen_inputs(

@@ -33,12 +33,21 @@ too, paged_kv_cuda.cu:168-171).  Additive ops, with no reference schema:
     store_gather(Tensor key, Tensor value, Tensor(a!) key_cache,
                  Tensor(b!) value_cache, Tensor slot_mapping, Tensor plan,
                  int num_seqs, Tensor(c!) key_out, Tensor(d!) value_out) -> ()
+    rotary(Tensor q, Tensor k, Tensor positions, Tensor table, int layout,
+           int[] section_ends, Tensor(a!) q_out, Tensor(b!) k_out) -> ()
+    rotary_store(Tensor q, Tensor k, Tensor v, Tensor(a!) key_cache,
+                 Tensor(b!) value_cache, Tensor slot_mapping, Tensor positions,
+                 Tensor table, int layout, int[] section_ends,
+                 Tensor(c!) q_out, Tensor(d!)? k_out=None) -> ()
+    copy_blocks(Tensor cache, Tensor(a!) dst, Tensor pairs) -> ()
 
 Every kernel runs on the current stream of the tensors' device and returns
 before it completes, like the reference ops.
 """
 from __future__ import annotations
 
+import ctypes
+import math
 from threading import Lock
 
 import torch
@@ -74,6 +83,12 @@ SCHEMAS = {
     "paged_attention_prefill": "paged_attention_prefill(Tensor q, Tensor key_cache, "
     "Tensor value_cache, Tensor block_tables, Tensor cu_seqlens_q, Tensor cu_seqlens_k, "
     "Tensor plan, float scale, Tensor(a!) out) -> ()",
+    "rotary": "rotary(Tensor q, Tensor k, Tensor positions, Tensor table, int layout, "
+    "int[] section_ends, Tensor(a!) q_out, Tensor(b!) k_out) -> ()",
+    "rotary_store": "rotary_store(Tensor q, Tensor k, Tensor v, Tensor(a!) key_cache, "
+    "Tensor(b!) value_cache, Tensor slot_mapping, Tensor positions, Tensor table, int layout, "
+    "int[] section_ends, Tensor(c!) q_out, Tensor(d!)? k_out=None) -> ()",
+    "copy_blocks": "copy_blocks(Tensor cache, Tensor(a!) dst, Tensor pairs) -> ()",
 }
 
 DTYPE_CODES = {
@@ -551,6 +566,129 @@ def _paged_attention_prefill_impl(q, key_cache, value_cache, block_tables, cu_se
     _lib.check(status, "nanovllm_paged_kv::paged_attention_prefill")
 
 
+def build_rotary_table(inv_freq: list[float], factor: float, max_position: int,
+                       device: torch.device) -> torch.Tensor:
+    """[max_position, len(inv_freq), 2] cosines and sines (fp32)."""
+    half = len(inv_freq)
+    with torch.cuda.device(device):
+        frequencies = torch.tensor(inv_freq, dtype=torch.float64, device=device)
+        table = torch.empty((max_position, half, 2), dtype=torch.float32, device=device)
+        status = _lib.load_library().nkv_rotary_table(
+            frequencies.data_ptr(), float(factor), max_position, 2 * half, table.data_ptr(),
+            _stream(device))
+    _lib.check(status, "nkv_rotary_table")
+    return table
+
+
+def _rotary_heads(name: str, x: torch.Tensor, tokens: int | None = None, like=None) -> None:
+    if x.ndim != 3 or (x.shape[2] > 1 and x.stride(2) != 1):
+        raise ValueError(f"rotary {name} must be [tokens, heads, head_dim] with a contiguous head_dim")
+    if tokens is not None and x.shape[0] != tokens:
+        raise ValueError(f"rotary {name} must have one row per token")
+    if like is not None and x.shape != like.shape:
+        raise ValueError(f"rotary {name} must have its input's shape")
+
+
+def _launch_rotary(q, k, v, key_cache, value_cache, slot_mapping, positions, table, layout: int,
+                   section_ends, q_out, k_out) -> None:
+    tensors = [t for t in (q, k, v, key_cache, value_cache, slot_mapping, positions, table, q_out,
+                           k_out) if t is not None]
+    device = _require_device("rotary positions", *tensors)
+    _rotary_heads("q", q)
+    tokens, q_heads, head_dim = q.shape
+    _rotary_heads("k", k, tokens)
+    if k.shape[2] != head_dim:
+        raise ValueError("rotary q and k must have the same head_dim")
+    _rotary_heads("q_out", q_out, like=q)
+    if k_out is not None:
+        _rotary_heads("k_out", k_out, like=k)
+    code = dtype_code(q.dtype)
+    if any(t is not None and t.dtype != q.dtype for t in (k, v, key_cache, value_cache, q_out, k_out)):
+        raise ValueError("rotary q, k, v, caches and outputs must have one dtype")
+    if (table.ndim != 3 or table.shape[2] != 2 or table.dtype != torch.float32
+            or not table.is_contiguous()):
+        raise ValueError("rotary table must be a contiguous [max_position, rotary_dim / 2, 2] float32 tensor")
+    half = table.shape[1]
+    if 2 * half > head_dim:
+        raise ValueError(f"rotary table turns {2 * half} dims, the heads have {head_dim}")
+    if positions.dtype not in (torch.int32, torch.int64) or positions.ndim not in (1, 2):
+        raise ValueError("positions must be int32 or int64, [tokens] or [3, tokens]")
+    if (positions.shape[-1] != tokens or (positions.ndim == 2 and positions.shape[0] != 3)
+            or (tokens > 1 and positions.stride(-1) != 1)):
+        raise ValueError("positions must be [tokens] or [3, tokens] with contiguous rows")
+    ends = tuple(int(e) for e in section_ends)
+    if len(ends) != 2:
+        raise ValueError("section_ends must hold two counts of pairs")
+    row_stride = 0
+    if positions.ndim == 2:
+        if ends == (half, half):
+            raise ValueError("three position rows need a rotary table with sections")
+        if positions.stride(0) < tokens:  # an expanded row: three rows of their own
+            positions = positions.contiguous()
+        row_stride = positions.stride(0)
+    d = _lib.RotaryDesc()
+    d.num_slots = 0
+    if key_cache is not None:
+        _require_contiguous_cache("rotary store", key_cache, value_cache)
+        slot_mapping = _int32_index("rotary store", "slot_mapping", slot_mapping)
+        _require_store_rows(k, v, key_cache, value_cache, slot_mapping)
+        d.v, d.v_token_stride, d.v_head_stride = v.data_ptr(), v.stride(0), v.stride(1)
+        d.key_cache, d.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
+        d.slot_mapping = slot_mapping.data_ptr()
+        d.num_slots = key_cache.shape[0] * key_cache.shape[1]
+    if tokens == 0:
+        return
+    d.q, d.q_token_stride, d.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
+    d.k, d.k_token_stride, d.k_head_stride = k.data_ptr(), k.stride(0), k.stride(1)
+    d.q_out, d.q_out_token_stride, d.q_out_head_stride = q_out.data_ptr(), q_out.stride(0), q_out.stride(1)
+    if k_out is not None:
+        d.k_out, d.k_out_token_stride, d.k_out_head_stride = (k_out.data_ptr(), k_out.stride(0),
+                                                              k_out.stride(1))
+    d.positions, d.position_bytes = positions.data_ptr(), positions.element_size()
+    d.position_row_stride = row_stride
+    d.section_ends[0], d.section_ends[1] = ends
+    d.table, d.max_position, d.rotary_dim = table.data_ptr(), table.shape[0], 2 * half
+    d.num_tokens, d.num_q_heads, d.num_kv_heads, d.head_dim = tokens, q_heads, k.shape[1], head_dim
+    d.layout, d.dtype = layout, code
+    with torch.cuda.device(device):
+        status = _lib.load_library().nkv_rotary(ctypes.byref(d), _stream(device))
+    _lib.check(status, "nanovllm_paged_kv::rotary")
+
+
+def _rotary_impl(q, k, positions, table, layout: int, section_ends, q_out, k_out) -> None:
+    _launch_rotary(q, k, None, None, None, None, positions, table, layout, section_ends, q_out, k_out)
+
+
+def _rotary_store_impl(q, k, v, key_cache, value_cache, slot_mapping, positions, table, layout: int,
+                       section_ends, q_out, k_out=None) -> None:
+    _launch_rotary(q, k, v, key_cache, value_cache, slot_mapping, positions, table, layout,
+                   section_ends, q_out, k_out)
+
+
+def _copy_blocks_impl(cache, dst, pairs) -> None:
+    device = _require_device("paged KV HIP block copy", cache, dst, pairs)
+    if cache.ndim < 4 or not cache.is_contiguous() or not dst.is_contiguous():
+        raise ValueError("block copy requires contiguous [.., blocks, block, kv_heads, head_dim] caches")
+    if (dst.dtype != cache.dtype or dst.shape[:-4] != cache.shape[:-4]
+            or dst.shape[-3:] != cache.shape[-3:]):
+        raise ValueError("block copy: the caches may differ in their number of blocks only")
+    if pairs.dtype != torch.int32 or pairs.ndim != 2 or pairs.shape[1] != 2 or not pairs.is_contiguous():
+        raise ValueError("block copy: pairs must be a contiguous [n, 2] int32 tensor")
+    dtype_code(cache.dtype)
+    a, b = cache.data_ptr(), dst.data_ptr()
+    size = cache.element_size()
+    if (a != b or cache.shape != dst.shape) and a < b + dst.numel() * size and b < a + cache.numel() * size:
+        raise ValueError("block copy: two caches must not overlap")
+    planes = math.prod(cache.shape[:-4])
+    if pairs.shape[0] == 0 or planes == 0 or cache.numel() == 0 or dst.numel() == 0:
+        return
+    with torch.cuda.device(device):
+        status = _lib.load_library().nkv_copy_blocks(
+            a, b, planes, cache.shape[-4], dst.shape[-4], math.prod(cache.shape[-3:]) * size,
+            pairs.data_ptr(), pairs.shape[0], _stream(device))
+    _lib.check(status, "nanovllm_paged_kv::copy_blocks")
+
+
 def register_ops() -> None:
     """Define the schemas (unless another library already did) and register
     the HIP implementations on the CUDA key.  Idempotent."""
@@ -574,6 +712,9 @@ def register_ops() -> None:
         fragment.impl("store_gather", _store_gather_impl, "CUDA")
         fragment.impl("build_prefill_plan", _build_prefill_plan_impl, "CUDA")
         fragment.impl("paged_attention_prefill", _paged_attention_prefill_impl, "CUDA")
+        fragment.impl("rotary", _rotary_impl, "CUDA")
+        fragment.impl("rotary_store", _rotary_store_impl, "CUDA")
+        fragment.impl("copy_blocks", _copy_blocks_impl, "CUDA")
         _FRAGMENT = fragment
 
 
@@ -591,3 +732,6 @@ build_prefill_plan = _build_prefill_plan_impl
 paged_attention_prefill = _paged_attention_prefill_impl
 build_store_gather_plan = _build_store_gather_plan_impl
 store_gather = _store_gather_impl
+rotary = _rotary_impl
+rotary_store = _rotary_store_impl
+copy_blocks = _copy_blocks_impl

@@ -64,6 +64,10 @@ class DeviceBlockPool:
         self._ops: list[tuple[int, int, int, int]] = []
         self._args: list[int] = []
         self._run: set[int] = set()
+        self._pairs = 0  # pages that the log's forks copy
+        self._freed = False  # whether a deallocation follows the log's first copying fork
+        self._copied: dict[int, int] = {}  # children of the log's copying forks: their block counts
+        self.copies = torch.empty((0, 2), dtype=torch.int32, device=self.device)
         self._staging: torch.Tensor | None = None
         self._uploaded: torch.cuda.Event | None = None
         self.reset()
@@ -82,6 +86,9 @@ class DeviceBlockPool:
         self._ops.clear()
         self._args.clear()
         self._run.clear()
+        self._pairs, self._freed = 0, False
+        self._copied.clear()
+        self.copies = self.copies[:0]
         _lib.check(_lib.load_library().nkv_pool_init(ctypes.byref(self._desc), self._stream()),
                    "nkv_pool_init")
 
@@ -111,6 +118,7 @@ class DeviceBlockPool:
         """BlockManager.deallocate (block_manager.py:216-227)."""
         slot = self._check_slot(slot)
         self._run.clear()
+        self._freed = self._freed or self._pairs > 0
         self._ops.append((_lib.NKV_POOL_OP_DEALLOCATE, slot, 0, 0))
 
     def append(self, slot: int) -> None:
@@ -131,6 +139,57 @@ class DeviceBlockPool:
             return True
         return False
 
+    # ------------------------------------- what BlockManager does not have
+    def fork(self, parent: int, child: int, num_tokens: int) -> None:
+        """`child` (empty) continues `parent`'s first `num_tokens` tokens:
+        their whole blocks are held once more, a partly filled last one is
+        replaced by a fresh block from the queue front, whose page has to be
+        copied: after flush(), `copies` lists these {source, destination}
+        pairs in the order of the forks
+        (``backend.copy_blocks(cache, pool.copies)``)."""
+        parent, child = self._check_slot(parent), self._check_slot(child)
+        num_tokens = int(num_tokens)
+        if parent == child:
+            raise ValueError("a sequence cannot be forked into its own slot")
+        blocks = -(-num_tokens // self.block_size)
+        if num_tokens < 0 or blocks > self.width:
+            raise ValueError("need 0 <= num_tokens <= max_blocks_per_seq blocks of tokens")
+        copied = num_tokens % self.block_size != 0
+        if copied and self._freed:
+            raise ValueError("the log frees blocks after a fork: flush and copy that fork's pages "
+                             "first, a freed source could become this fork's destination")
+        if copied and self._copied.get(parent) == blocks:
+            raise ValueError("the log forks a fork at its copied page: fork its parent, or flush and "
+                             "copy the pages first")
+        if copied:
+            self._copied[child] = blocks
+        self._run.clear()
+        self._ops.append((_lib.NKV_POOL_OP_FORK, child, blocks, len(self._args)))
+        self._args.extend((parent, self._pairs if copied else -1))
+        self._pairs += 1 if copied else 0
+
+    def compact(self) -> torch.Tensor:
+        """Applies the log, then moves the blocks in use to the low ids: of U
+        of them, the k-th at or past U to the k-th free one below.  Tables
+        and reference counts follow, the free queue becomes U, U + 1, ...
+        Returns the moves as [n, 2] int32 pairs {old, new} on the device,
+        for ``backend.copy_blocks(cache, moves)`` and for the caller's own
+        block ids (its prefix hashes).  Reads their number back (one
+        synchronisation).  Pages that earlier forks copy must have been
+        copied: with any in the log, flush and copy first."""
+        if self._pairs:
+            raise ValueError("the log holds forks whose pages are not copied: flush and copy them first")
+        self._run.clear()
+        self._ops.append((_lib.NKV_POOL_OP_COMPACT, 0, 0, len(self._args)))
+        self._args.append(0)
+        moves = torch.empty((max(1, self.num_blocks // 2), 2), dtype=torch.int32, device=self.device)
+        self._flush(moves)
+        meta = self.meta.cpu().tolist()
+        if meta[4]:
+            raise RuntimeError(f"block pool op {int(meta[3]) - 1} failed: "
+                               f"{_lib.NKV_POOL_ERRORS.get(int(meta[4]), '?')} (code {int(meta[4])})")
+        return moves[: int(meta[5])]
+
     @property
     def pending_ops(self) -> int:
         return len(self._ops)
@@ -142,6 +201,11 @@ class DeviceBlockPool:
         nanokv.benchmark.LaunchTimer) brackets the apply kernel alone."""
         if not self._ops:
             return
+        copies = torch.full((self._pairs, 2), -1, dtype=torch.int32, device=self.device)
+        self._flush(copies, timer)
+        self.copies = copies
+
+    def _flush(self, copies: torch.Tensor, timer=None) -> None:
         ops = np.asarray(self._ops, dtype=np.int32).reshape(-1)
         args = np.asarray(self._args, dtype=np.int32)
         total = ops.size + max(args.size, 1)
@@ -158,9 +222,10 @@ class DeviceBlockPool:
             self._uploaded = torch.cuda.Event()
         self._uploaded.record(torch.cuda.current_stream(self.device))
         started = timer.start() if timer is not None else None
-        status = _lib.load_library().nkv_pool_apply(
+        status = _lib.load_library().nkv_pool_apply_copies(
             ctypes.byref(self._desc), device_log.data_ptr(), len(self._ops),
-            device_log[ops.size:].data_ptr(), args.size, self._stream(),
+            device_log[ops.size:].data_ptr(), args.size,
+            copies.data_ptr() if copies.numel() else None, copies.shape[0], self._stream(),
         )
         if timer is not None:
             timer.stop(started)
@@ -168,6 +233,8 @@ class DeviceBlockPool:
         self._ops.clear()
         self._args.clear()
         self._run.clear()
+        self._pairs, self._freed = 0, False
+        self._copied.clear()
 
     # ---------------------------------------------------------------- reads
     def error(self) -> tuple[int, int, str] | None:

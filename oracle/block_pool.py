@@ -83,6 +83,35 @@ class BlockPoolOracle:
         table.append(block_id)
         return block_id
 
+    # -- without a counterpart in the reference
+    def fork(self, parent: int, child: int, blocks: int, copied: bool) -> tuple[int, int] | None:
+        """`child` holds `parent`'s first `blocks` blocks once more each, the
+        last replaced by a fresh one when `copied`; returns the page to copy."""
+        assert not self.tables.get(child) and parent != child
+        table = list(self.tables.get(parent, [])[:blocks])
+        assert len(table) == blocks and not (copied and not blocks)
+        pair = None
+        if copied:
+            pair = (table[-1], self._allocate_block())
+            table[-1] = pair[1]
+        for block_id in table[:-1] if copied else table:
+            self.ref[block_id] += 1
+        self.tables[child] = table
+        return pair
+
+    def compact(self) -> list[tuple[int, int]]:
+        used = [b for b in range(self.num_blocks) if self.ref[b] > 0]
+        low = len(used)
+        holes = [b for b in range(low) if self.ref[b] == 0]
+        moves = list(zip([b for b in used if b >= low], holes))
+        assert len(moves) == len(holes)
+        name = dict(moves)
+        for old, new in moves:
+            self.ref[new], self.ref[old] = self.ref[old], 0
+        self.tables = {s: [name.get(b, b) for b in t] for s, t in self.tables.items()}
+        self.free = deque(range(low, self.num_blocks))
+        return moves
+
     # -- views
     def queue(self) -> list[int]:
         return list(self.free)
