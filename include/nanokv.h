@@ -711,6 +711,49 @@ int nkv_rotary_table(const double* inv_freq, double factor, int64_t max_position
                      int64_t rotary_dim, float* table, void* stream);
 int nkv_rotary(const nkv_rotary_desc* desc, void* stream);
 
+/*
+ * Paged-attention decode of a batch whose sequences share prefixes: as
+ * nkv_paged_attention_decode, with the prefix of a group of sequences read
+ * once for all of its query rows.  Group g is the sequences [cu_groups[g],
+ * cu_groups[g+1]); the first prefix_lens[g] rows of their contexts are the
+ * same (the same blocks, or the same contents) and are read through the
+ * block table of the group's first sequence.  Groups of one sequence, groups
+ * with no prefix, sequences in no group and sequences shorter than their
+ * group's prefix share nothing and are read through their own tables.
+ * Scores, weights' sums and outputs are held in fp32 and rounded once; the
+ * weights are rounded to the input type before the product with V.
+ * dtype, head_dim, heads, tables, q, out and scale as
+ * nkv_paged_attention_decode has them.  No counterpart in the reference.
+ *
+ * nkv_build_shared_plan writes nkv_shared_plan_bytes(...) bytes (16-byte
+ *   aligned); one plan serves every layer of a step.  rest_tokens is the sum
+ *   of what the sequences do not share, or an upper bound of it (-1:
+ *   unknown); it bounds the launch and the workspace, and a sum above it is
+ *   served all the same.  A plan for another batch size, group count or head
+ *   layout gives NaN in every output.
+ * The attention call takes the same counts, and a workspace of
+ *   nkv_shared_workspace_bytes(...) bytes (16-byte aligned).
+ */
+int64_t nkv_shared_plan_bytes(int64_t num_seqs, int64_t num_groups,
+                              int64_t num_kv_heads, int64_t num_q_heads,
+                              int64_t rest_tokens);
+int64_t nkv_shared_workspace_bytes(int64_t num_seqs, int64_t num_groups,
+                                   int64_t num_kv_heads, int64_t num_q_heads,
+                                   int64_t rest_tokens);
+int nkv_build_shared_plan(const int32_t* cu_seqlens_k, int64_t num_seqs,
+                          const int32_t* cu_groups, const int32_t* prefix_lens,
+                          int64_t num_groups, int64_t num_kv_heads,
+                          int64_t num_q_heads, int64_t rest_tokens, void* plan,
+                          int64_t plan_bytes, void* stream);
+int nkv_shared_prefix_attention_decode(
+    const void* q, int64_t q_seq_stride, const void* key_cache,
+    const void* value_cache, const int32_t* block_tables, int64_t table_stride,
+    const void* plan, int64_t plan_bytes, int64_t num_seqs, int64_t num_groups,
+    int64_t num_kv_heads, int64_t num_q_heads, int64_t head_dim,
+    int64_t block_size, int64_t num_blocks, int64_t rest_tokens, float scale,
+    int32_t dtype, void* workspace, int64_t workspace_bytes, void* out,
+    int64_t out_seq_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

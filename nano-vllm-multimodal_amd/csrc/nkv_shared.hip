@@ -1,0 +1,925 @@
+// Decode attention of a batch whose sequences share prefixes: one query
+// token per sequence over its paged context, as nkv_attention.hip computes
+// it, but the prefix that a group of consecutive sequences has in common is
+// read once for all of the group's query rows.
+//
+// Group g (sequences [cu_groups[g], cu_groups[g+1])) shares the first P_g
+// rows of its contexts.  For the (sequence, query head) rows of one kv head
+//   o = (sum_prefix w v + sum_rest w v) / (sum_prefix w + sum_rest w),
+//   w = exp(scale q k - m),
+// the prefix sums of all rows of the group are one product of the rows with
+// the prefix's keys and one with its values; the sums over the rest of each
+// context are a sequence's own.  Both are cut into pieces of keys whose
+// partials (m, weight sum, 128 output sums, all fp32) a merge adds up.
+//
+// One launch holds both kinds of items, the prefix's first: they are bound
+// by the matrix cores, the others by HBM, so they run side by side on a CU.
+// An item is one workgroup of four wavefronts over 64-key tiles in LDS,
+// double-buffered and copied straight from the cache (global_load_lds).  RW
+// of its wavefronts split the query rows (32 each), 4 / RW the keys of a
+// tile; a group with few rows splits keys only, as does a sequence's rest
+// (16 rows: the query heads of a kv head), and then every wavefront reads
+// only the keys it copied itself, so its loop has no barrier.
+//   S^T = K Q^T    16x16x32 MFMAs: a lane's scores belong to one query row
+//   O^T += V^T P^T the weights, rounded to the element type, straight from
+//                  the score registers; V^T from the transposing LDS read;
+//                  a product with ones sums the same rounded weights.
+// Sequences shorter than their group's prefix share nothing and are read
+// from row 0 through their own table, so no row is masked inside a tile.
+// Keys in a block outside the cache or past the table are dropped: they copy
+// a row of zeros and their scores become -inf.
+#include <algorithm>
+#include <cmath>
+
+#include "nkv_common.h"
+#include "nkv_mfma.h"
+
+namespace nkv {
+namespace {
+
+constexpr int kDim = 128;
+constexpr int kThreads = 256;
+constexpr int kTileKeys = 64;
+constexpr int kChunk = 16;        // keys a wavefront copies per tile
+constexpr int kMaxGroup = 16;     // query heads per kv head
+constexpr int kEntryRows = 128;   // partial rows kept per prefix entry and kv head
+constexpr int kPlanThreads = 1024;
+constexpr int kSlots = 512;       // workgroups resident on the chip: two per CU
+constexpr int kRestRounds = 4;    // entries of the rests: at most so many rounds of workgroups
+constexpr int kMinPrefixTiles = 2;
+constexpr int kMinRestTiles = 2;
+constexpr float kRescaleLog2 = 8.f;  // the reference max moves only past this
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(4))) const int32_t const_i32;
+
+// ------------------------------------------------------------------ the plan
+//
+// int4s:
+//   [0]  {prefix entries, rest entries, num_seqs, num_groups}
+//   [1]  {num_kv_heads, query heads per kv head, 0, 0}
+//   [2, 18)  256 bytes of zeros, the row that dropped keys copy
+//   two per sequence  {rest's first row, context length, first rest entry, rest entries}
+//                     {first entry of its group's first tile, pieces per tile, member, log2 tile rows}
+//   two per prefix entry  {first sequence, first query row, query rows, log2 tile rows}
+//                         {first key, past the last, 0, 0}
+//   one per rest entry  {sequence, first row, past the last, 0}
+// The query rows of a group and kv head are member-major, (member, head).
+constexpr int kPlanSeqs = 18;
+struct PlanShape {
+  int64_t seqs, prefix, rest;  // sequences and entries to allocate
+  __host__ __device__ int64_t prefix_at() const { return kPlanSeqs + 2 * seqs; }
+  __host__ __device__ int64_t rest_at() const { return prefix_at() + 2 * prefix; }
+  __host__ __device__ int64_t int4s() const { return rest_at() + rest; }
+  __host__ __device__ int64_t prefix_rows(int64_t kv_heads) const { return prefix * kv_heads * kEntryRows; }
+  __host__ __device__ int64_t rows(int64_t kv_heads, int64_t group) const {
+    return prefix_rows(kv_heads) + rest * kv_heads * group;
+  }
+};
+__host__ __device__ constexpr int64_t slots_per_head(int64_t kv_heads) {
+  return kSlots / kv_heads > 0 ? kSlots / kv_heads : 1;
+}
+// A prefix has one tile of rows or one per 128 of them, cut into at most
+// slots pieces beside one per tile; a rest one entry beside its share.
+PlanShape plan_shape(int64_t num_seqs, int64_t num_groups, int64_t kv_heads, int64_t group,
+                     int64_t rest_tokens) {
+  PlanShape p{num_seqs, 0, 0};
+  const int64_t sharing = std::min(num_groups, num_seqs / 2);
+  if (sharing > 0) p.prefix = slots_per_head(kv_heads) + sharing + num_seqs * group / kEntryRows;
+  p.rest = slots_per_head(kv_heads) * kRestRounds;
+  if (rest_tokens >= 0) p.rest = std::min(p.rest, rest_tokens / kChunk + 1);
+  p.rest += num_seqs;
+  return p;
+}
+
+__device__ __forceinline__ int32_t tile_log2(int64_t rows) {  // query rows per tile: 16, 32, 64 or 128
+  return rows <= 16 ? 4 : rows <= 32 ? 5 : rows <= 64 ? 6 : 7;
+}
+
+__device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* s_sum) {
+#pragma unroll
+  for (int d = kWave / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, kWave);
+  __syncthreads();
+  if (threadIdx.x % kWave == 0) s_sum[threadIdx.x / kWave] = v;
+  __syncthreads();
+  int64_t total = 0;
+  for (int w = 0; w < kPlanThreads / kWave; ++w) total += s_sum[w];
+  return total;
+}
+
+struct GroupOf {
+  const int32_t* cu;
+  const int32_t* prefix;
+  int32_t num_groups, num_seqs;
+  // A group that shares something: at least two sequences of the batch.
+  __device__ __forceinline__ bool shares(int32_t g, int32_t* first, int32_t* n, int32_t* rows) const {
+    const int32_t s0 = cu[g], s1 = cu[g + 1];
+    *first = s0;
+    *n = s1 - s0;
+    *rows = prefix[g];
+    return s0 >= 0 && s1 <= num_seqs && s1 - s0 >= 2 && *rows > 0;
+  }
+  // The group of sequence i, -1 for none.
+  __device__ __forceinline__ int32_t of(int32_t i) const {
+    int32_t lo = 0, hi = num_groups;
+    while (hi - lo > 1) {
+      const int32_t mid = (lo + hi) >> 1;
+      if (cu[mid] <= i) {
+        lo = mid;
+      } else {
+        hi = mid;
+      }
+    }
+    // Empty groups at the same place: the last one that starts at or before i.
+    return num_groups > 0 && cu[lo] <= i && i < cu[lo + 1] ? lo : -1;
+  }
+};
+
+__global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
+    const int32_t* __restrict__ cu_seqlens_k, GroupOf groups, int32_t num_kv_heads, int32_t group,
+    PlanShape shape, int4* __restrict__ plan) {
+  extern __shared__ int32_t s_mem[];
+  __shared__ int64_t s_sum[kPlanThreads / kWave];
+  __shared__ int32_t s_tmp[kPlanThreads / kWave + 1];
+  const int32_t t = threadIdx.x;
+  const int32_t num_seqs = groups.num_seqs;
+  const int32_t num_groups = groups.num_groups;
+  // Where sequence i's own part begins: its group's prefix, when it has all of it.
+  auto rest_of = [&](int32_t i, int32_t* length) {
+    *length = max(0, cu_seqlens_k[i + 1] - cu_seqlens_k[i]);
+    const int32_t g = groups.of(i);
+    int32_t first, n, rows;
+    return g >= 0 && groups.shares(g, &first, &n, &rows) && *length >= rows ? rows : 0;
+  };
+
+  int64_t prefix_units = 0, rest_units = 0;  // 64-key tiles to walk, per kv head
+  for (int32_t g = t; g < num_groups; g += kPlanThreads) {
+    int32_t first, n, rows;
+    if (groups.shares(g, &first, &n, &rows)) {
+      const int64_t q_rows = static_cast<int64_t>(n) * group;
+      const int64_t tiles = (q_rows + kEntryRows - 1) / kEntryRows;
+      prefix_units += tiles * ((static_cast<int64_t>(rows) + kTileKeys - 1) / kTileKeys);
+    }
+  }
+  for (int32_t i = t; i < num_seqs; i += kPlanThreads) {
+    int32_t length;
+    const int32_t start = rest_of(i, &length);
+    if (length > start) rest_units += (static_cast<int64_t>(length) - (start & -kChunk) + kTileKeys - 1) / kTileKeys;
+  }
+  prefix_units = block_sum(prefix_units, s_sum);
+  rest_units = block_sum(rest_units, s_sum);
+  // Tiles per piece: all items together one round of workgroups.  The rests'
+  // entries are bounded by the plan's room for them.
+  const int64_t slots = slots_per_head(num_kv_heads);
+  const int64_t share = (prefix_units + rest_units + slots - 1) / slots;
+  const int64_t prefix_tiles = max(static_cast<int64_t>(kMinPrefixTiles), share);
+  const int64_t room = max(static_cast<int64_t>(1), shape.rest - num_seqs);
+  const int64_t rest_tiles =
+      max(max(static_cast<int64_t>(kMinRestTiles), share), (rest_units + room - 1) / room);
+  const int32_t piece_keys = static_cast<int32_t>(min(prefix_tiles, static_cast<int64_t>(1) << 24) * kTileKeys);
+  const int32_t entry_keys = static_cast<int32_t>(min(rest_tiles, static_cast<int64_t>(1) << 24) * kTileKeys);
+
+  // Prefix entries: a group's tiles of query rows, each cut into pieces.
+  lds_exclusive_scan<kPlanThreads>(
+      num_groups,
+      [&](int32_t g) {
+        int32_t first, n, rows;
+        if (!groups.shares(g, &first, &n, &rows)) return 0;
+        const int32_t tiles = (n * group + kEntryRows - 1) / kEntryRows;
+        return tiles * ((rows - 1) / piece_keys + 1);
+      },
+      s_mem, s_tmp);
+  const int32_t prefix_entries = static_cast<int32_t>(min(static_cast<int64_t>(s_mem[num_groups]), shape.prefix));
+  for (int32_t e = t; e < prefix_entries; e += kPlanThreads) {
+    const int32_t g = owner_of(s_mem, num_groups, e);
+    int32_t first, n, rows;
+    groups.shares(g, &first, &n, &rows);
+    const int32_t pieces = (rows - 1) / piece_keys + 1;
+    const int32_t tile = (e - s_mem[g]) / pieces, piece = (e - s_mem[g]) % pieces;
+    const int32_t log2 = tile_log2(static_cast<int64_t>(n) * group);
+    // Pieces of equal length, in whole tiles.
+    const int32_t key_tiles = (rows - 1) / kTileKeys + 1;
+    const int32_t k0 = static_cast<int32_t>(static_cast<int64_t>(key_tiles) * piece / pieces) * kTileKeys;
+    const int32_t k1 = min(rows, static_cast<int32_t>(static_cast<int64_t>(key_tiles) * (piece + 1) / pieces) * kTileKeys);
+    plan[shape.prefix_at() + 2 * e] =
+        make_int4(first, tile * kEntryRows, min(kEntryRows, n * group - tile * kEntryRows), log2);
+    plan[shape.prefix_at() + 2 * e + 1] = make_int4(k0, k1, 0, 0);
+  }
+  for (int32_t i = t; i < num_seqs; i += kPlanThreads) {
+    const int32_t g = groups.of(i);
+    int32_t first, n, rows, length;
+    int4 record = make_int4(0, 0, 0, 0);
+    if (rest_of(i, &length) > 0) {
+      groups.shares(g, &first, &n, &rows);
+      record = make_int4(s_mem[g], (rows - 1) / piece_keys + 1, i - first,
+                         tile_log2(static_cast<int64_t>(n) * group));
+    }
+    plan[kPlanSeqs + 2 * i + 1] = record;
+  }
+  __syncthreads();
+  // The rests.
+  lds_exclusive_scan<kPlanThreads>(
+      num_seqs,
+      [&](int32_t i) {
+        int32_t length;
+        const int32_t start = rest_of(i, &length);
+        return length > start ? (length - (start & -kChunk) - 1) / entry_keys + 1 : 0;
+      },
+      s_mem, s_tmp);
+  const int32_t rest_entries = static_cast<int32_t>(min(static_cast<int64_t>(s_mem[num_seqs]), shape.rest));
+  for (int32_t i = t; i < num_seqs; i += kPlanThreads) {
+    int32_t length;
+    const int32_t start = rest_of(i, &length);
+    plan[kPlanSeqs + 2 * i] = make_int4(start, length, s_mem[i], s_mem[i + 1] - s_mem[i]);
+  }
+  for (int32_t e = t; e < rest_entries; e += kPlanThreads) {
+    const int32_t i = owner_of(s_mem, num_seqs, e);
+    int32_t length;
+    const int32_t start = rest_of(i, &length);
+    const int32_t row0 = (start & -kChunk) + (e - s_mem[i]) * entry_keys;  // cuts at whole chunks
+    plan[shape.rest_at() + e] =
+        make_int4(i, max(start, row0), length - row0 > entry_keys ? row0 + entry_keys : length, 0);
+  }
+  if (t < 16) plan[2 + t] = make_int4(0, 0, 0, 0);
+  if (t == 0) {
+    plan[0] = make_int4(prefix_entries, rest_entries, num_seqs, num_groups);
+    plan[1] = make_int4(num_kv_heads, group, 0, 0);
+  }
+}
+
+// ------------------------------------------------------------- the attention
+
+template <int N>
+__device__ __forceinline__ void wait_vmcnt() {
+  asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lgkmcnt0() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
+
+struct TileShared {
+  u32x4 k[2][kTileKeys * 16];
+  u32x4 v[2][kTileKeys * 16];
+  float m[4][32];
+  float l[4][32];
+};
+
+// The cache as one item sees it: a kv head of the rows of one block table.
+struct KeySource {
+  const uint8_t* k_head;
+  const uint8_t* v_head;
+  const const_i32* table;
+  const uint8_t* zeros;
+  int64_t table_stride;
+  uint32_t row_bytes;
+  int32_t block_size, block_shift, num_blocks;
+  int32_t begin, end;  // context rows; tiles start at begin rounded down to a chunk
+};
+
+// The item's query rows [row0, row0 + rows): row r is head r % group of the
+// sequence first + r / group.
+struct RowSource {
+  const uint16_t* q;  // of the kv head's first query head
+  int64_t seq_stride;
+  int32_t first, row0, rows, group;
+};
+
+// kChunked: blocks are whole 16-key chunks (one block id per chunk, read as a
+// scalar); otherwise every key looks up its own.
+template <int RW, int NMB, bool kChunked, bool kHalf>
+__device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, const RowSource& rows,
+                                       float scale_log2, float* __restrict__ part_acc,
+                                       f32x2* __restrict__ part_ml) {
+  typedef Elem<kHalf> E;
+  typedef typename E::T T;
+  typedef typename E::X8 X8;
+  typedef typename E::X4 X4;
+  constexpr int KW = 4 / RW;
+  constexpr int NKB = RW;  // 16-key blocks a wavefront computes per tile
+  static_assert(RW == 1 || NMB == 2, "row waves hold 32 rows");
+  const int tid = threadIdx.x;
+  const int lane = tid & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int c16 = lane & 15;
+  const int g4 = lane >> 4;
+  const int rw = wave % RW;   // which 32 rows
+  const int kw = wave / RW;   // which keys of a tile
+  const int chunk = kw * NKB + rw;  // the 16 keys this wavefront copies
+
+  // Q^T operands: row 16 mb + c16 of the wavefront's, dims 32 dc + 8 g4 .. +8.
+  X8 qb[NMB][4];
+#pragma unroll
+  for (int mb = 0; mb < NMB; ++mb) {
+    const int32_t r = rows.row0 + rw * 32 + mb * 16 + c16;
+    const bool ok = rw * 32 + mb * 16 + c16 < rows.rows;
+    const int32_t member = ok ? r / rows.group : 0;
+    const int32_t head = ok ? r - member * rows.group : 0;
+    const uint16_t* row = rows.q + static_cast<int64_t>(rows.first + member) * rows.seq_stride + head * kDim;
+#pragma unroll
+    for (int dc = 0; dc < 4; ++dc) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (ok) v = *reinterpret_cast<const u32x4*>(row + 32 * dc + 8 * g4);
+      qb[mb][dc] = __builtin_bit_cast(X8, v);
+    }
+  }
+
+  // The block id of context row t, -1 outside the item, table or cache.
+  auto block_of = [&](int32_t t) -> int32_t {
+    const int32_t logical = src.block_shift >= 0 ? t >> src.block_shift : t / src.block_size;
+    if (logical >= src.table_stride) return -1;
+    const int32_t id = src.table[logical];
+    return id >= 0 && id < src.num_blocks ? id : -1;
+  };
+  auto offset_in_block = [&](int32_t t) -> int32_t {
+    return src.block_shift >= 0 ? t & (src.block_size - 1) : t % src.block_size;
+  };
+  // Which of the 16 keys from t on are there (bit = key).
+  auto keys_there = [&](int32_t t) -> uint32_t {
+    if constexpr (kChunked) {
+      if (t >= src.end || block_of(t) < 0) return 0u;
+      const int32_t low = max(0, src.begin - t), high = min(kChunk, src.end - t);
+      return ((1u << high) - 1u) & ~((1u << low) - 1u);
+    } else {
+      const bool ok = t + c16 >= src.begin && t + c16 < src.end && block_of(t + c16) >= 0;
+      return static_cast<uint32_t>(__ballot(ok)) & 0xFFFFu;  // lanes 0-15
+    }
+  };
+
+  const uint32_t lds_k = lds_address(&sh.k[0][0]) + chunk * 4096u;
+  const uint32_t lds_v = lds_address(&sh.v[0][0]) + chunk * 4096u;
+  // Lane l copies 16 bytes of key 4 i + l / 16 to position l % 16 of its row.
+  uint32_t off_k[4], off_v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int key = 4 * i + g4;
+    off_k[i] = key * src.row_bytes + 16u * static_cast<uint32_t>(c16 ^ key);
+    off_v[i] = key * src.row_bytes + 16u * static_cast<uint32_t>(c16 ^ ((key & 7) << 1));
+  }
+  uint32_t there_next[NKB];
+  // Eight copies into buffer `slot`: this wavefront's chunk of the tile at t.
+  auto issue = [&](int slot, int32_t tile_t) {
+    const int32_t t = tile_t + chunk * kChunk;
+    const uint32_t dk = lds_k + slot * (kTileKeys * 256u), dv = lds_v + slot * (kTileKeys * 256u);
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) there_next[kb] = keys_there(tile_t + (kw * NKB + kb) * kChunk);
+    uint32_t there = there_next[0];
+#pragma unroll
+    for (int kb = 1; kb < NKB; ++kb) there = rw == kb ? there_next[kb] : there;
+    if (kChunked && there == 0xFFFFu) {
+      const int64_t row = static_cast<int64_t>(block_of(t)) * src.block_size + offset_in_block(t);
+      const uint8_t* const kr = src.k_head + row * src.row_bytes;
+      const uint8_t* const vr = src.v_head + row * src.row_bytes;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lds_copy16<true>(kr, off_k[i], dk + i * 1024u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) lds_copy16<true>(vr, off_v[i], dv + i * 1024u);
+    } else {
+      int64_t base[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 4 * i + g4;
+        const bool ok = (there >> key) & 1u;
+        const int32_t tk = ok ? t + key : 0;
+        const int32_t id = ok ? block_of(tk) : 0;
+        base[i] = ok ? (static_cast<int64_t>(id) * src.block_size + offset_in_block(tk)) *
+                           static_cast<int64_t>(src.row_bytes)
+                     : -1;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 4 * i + g4;
+        const uint8_t* kr = base[i] >= 0 ? src.k_head + base[i] : src.zeros;
+        lds_copy16<true>(kr + 16 * (c16 ^ key), dk + i * 1024u);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 4 * i + g4;
+        const uint8_t* vr = base[i] >= 0 ? src.v_head + base[i] : src.zeros;
+        lds_copy16<true>(vr + 16 * (c16 ^ ((key & 7) << 1)), dv + i * 1024u);
+      }
+    }
+  };
+
+  float row_max[NMB];
+  f32x4 acc[9][NMB];  // dims 16 db + 4 g4 + i of row c16; block 8: the weight sum (g4 == 0, i == 0)
+#pragma unroll
+  for (int mb = 0; mb < NMB; ++mb) {
+    row_max[mb] = -INFINITY;
+#pragma unroll
+    for (int db = 0; db < 9; ++db) acc[db][mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const T one = c16 == 0 ? static_cast<T>(1.f) : static_cast<T>(0.f);
+  const int tr_key = 4 * g4 + ((lane >> 2) & 3);
+  const int tr_dim = 4 * (lane & 3);
+
+  const int32_t first_key = src.begin & ~(kChunk - 1);
+  const int32_t num_tiles = (src.end - first_key + kTileKeys - 1) / kTileKeys;
+  __builtin_amdgcn_s_waitcnt(0);  // q has landed: only the copies are in flight below
+  issue(0, first_key);
+  for (int32_t tile = 0; tile < num_tiles; ++tile) {
+    uint32_t there[NKB];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) there[kb] = there_next[kb];
+    if constexpr (RW == 1) {
+      if (tile + 1 < num_tiles) {
+        wait_lgkmcnt0();  // the other buffer has been read
+        issue((tile + 1) & 1, first_key + (tile + 1) * kTileKeys);
+        wait_vmcnt<8>();
+      } else {
+        wait_vmcnt<0>();
+      }
+    } else {
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();  // everyone's copies have landed, the other buffer has been read
+      if (tile + 1 < num_tiles) issue((tile + 1) & 1, first_key + (tile + 1) * kTileKeys);
+    }
+    const u32x4* const k_tile = sh.k[tile & 1];
+    const u32x4* const v_tile = sh.v[tile & 1];
+
+    f32x4 st[NKB][NMB];
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) {
+#pragma unroll
+      for (int mb = 0; mb < NMB; ++mb) st[kb][mb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int dc = 0; dc < 4; ++dc) {
+        const X8 a = __builtin_bit_cast(X8, k_tile[k_index(16 * (kw * NKB + kb) + c16, 4 * dc + g4)]);
+#pragma unroll
+        for (int mb = 0; mb < NMB; ++mb) st[kb][mb] = E::mfma(a, qb[mb][dc], st[kb][mb]);
+      }
+    }
+    uint32_t all = 0xFFFFu;
+#pragma unroll
+    for (int kb = 0; kb < NKB; ++kb) all &= there[kb];
+    if (all != 0xFFFFu) {
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int mb = 0; mb < NMB; ++mb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            st[kb][mb][i] = (there[kb] >> (4 * g4 + i)) & 1u ? st[kb][mb][i] : -INFINITY;
+          }
+    }
+    float ref[NMB];
+#pragma unroll
+    for (int mb = 0; mb < NMB; ++mb) {
+      float local = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) local = fmaxf(local, st[kb][mb][i]);
+      local = row4_max(local) * scale_log2;  // scale > 0: the max commutes with it
+      const bool move = local > row_max[mb] + kRescaleLog2;
+      if (__any(move)) {
+        const float m_new = move ? local : row_max[mb];
+        const float alpha = move ? __builtin_amdgcn_exp2f(row_max[mb] - m_new) : 1.f;
+#pragma unroll
+        for (int db = 0; db < 9; ++db) acc[db][mb] *= alpha;
+        row_max[mb] = m_new;
+      }
+      ref[mb] = row_max[mb] == -INFINITY ? INFINITY : row_max[mb];  // nothing yet: weights 0
+    }
+    if constexpr (NKB == 1) {
+      const X4 ones = {one, one, one, one};
+      X4 pb[NMB];
+#pragma unroll
+      for (int mb = 0; mb < NMB; ++mb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pb[mb][i] = static_cast<T>(
+              __builtin_amdgcn_exp2f(__builtin_fmaf(st[0][mb][i], scale_log2, -ref[mb])));
+        }
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        const X4 a = __builtin_bit_cast(X4, v_tr_read(v_tile, 16 * kw + tr_key, 16 * db + tr_dim));
+#pragma unroll
+        for (int mb = 0; mb < NMB; ++mb) acc[db][mb] = E::mfma16(a, pb[mb], acc[db][mb]);
+      }
+#pragma unroll
+      for (int mb = 0; mb < NMB; ++mb) acc[8][mb] = E::mfma16(ones, pb[mb], acc[8][mb]);
+    } else {
+      const X8 ones = {one, one, one, one, one, one, one, one};
+      X8 pb[NKB / 2][NMB];
+#pragma unroll
+      for (int mb = 0; mb < NMB; ++mb)
+#pragma unroll
+        for (int c = 0; c < NKB / 2; ++c) {
+          X8 w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            w[i] = static_cast<T>(
+                __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * c][mb][i], scale_log2, -ref[mb])));
+            w[4 + i] = static_cast<T>(
+                __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * c + 1][mb][i], scale_log2, -ref[mb])));
+          }
+          pb[c][mb] = w;
+        }
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+#pragma unroll
+        for (int c = 0; c < NKB / 2; ++c) {
+          const int key = 16 * kw * NKB + 32 * c + tr_key;
+          const u32x2 lo = v_tr_read(v_tile, key, 16 * db + tr_dim);
+          const u32x2 hi = v_tr_read(v_tile, key + 16, 16 * db + tr_dim);
+          const X8 a = __builtin_bit_cast(X8, u32x4{lo.x, lo.y, hi.x, hi.y});
+#pragma unroll
+          for (int mb = 0; mb < NMB; ++mb) acc[db][mb] = E::mfma(a, pb[c][mb], acc[db][mb]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < NKB / 2; ++c)
+#pragma unroll
+        for (int mb = 0; mb < NMB; ++mb) acc[8][mb] = E::mfma(ones, pb[c][mb], acc[8][mb]);
+    }
+  }
+
+  if constexpr (KW == 1) {
+#pragma unroll
+    for (int mb = 0; mb < NMB; ++mb) {
+      const int r = rw * 32 + mb * 16 + c16;
+      if (r >= rows.rows) continue;
+      float* dst = part_acc + static_cast<int64_t>(r) * kDim + 4 * g4;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(dst + 16 * db) = acc[db][mb];
+      if (g4 == 0) part_ml[r] = f32x2{row_max[mb], acc[8][mb][0]};
+    }
+  } else {
+    // The key waves add up through LDS: wavefront (rw, kw) leaves its rows in
+    // the buffers (16 KiB per wavefront, 16-byte pieces swizzled by row).
+    __syncthreads();  // every wavefront has read its last tile
+    u32x4* const buffers = reinterpret_cast<u32x4*>(&sh);  // k and v: 64 KiB in a row
+    u32x4* const buffer = buffers + wave * 1024;
+#pragma unroll
+    for (int mb = 0; mb < NMB; ++mb) {
+      const int r = mb * 16 + c16;
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        buffer[r * 32 + ((4 * db + g4) ^ c16)] = __builtin_bit_cast(u32x4, acc[db][mb]);
+      }
+      if (g4 == 0) {
+        sh.m[wave][r] = row_max[mb];
+        sh.l[wave][r] = acc[8][mb][0];
+      }
+    }
+    __syncthreads();
+    const int total_rows = min(rows.rows, RW * NMB * 16);
+    for (int idx = tid; idx < total_rows * 32; idx += kThreads) {
+      const int row = idx >> 5, piece = idx & 31;
+      const int from = row / 32, r = row & 31;  // row wave and its row
+      float top = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) top = fmaxf(top, sh.m[k * RW + from][r]);
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      float l = 0.f;
+#pragma unroll
+      for (int k = 0; k < KW; ++k) {
+        const int w = k * RW + from;
+        const float mw = sh.m[w][r], lw = sh.l[w][r];
+        // A wavefront without keys has (-inf, 0); -inf with another sum is
+        // NaN scores, which go on.
+        const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mw - top);
+        const f32x4 v = __builtin_bit_cast(f32x4, buffers[w * 1024 + r * 32 + (piece ^ (r & 15))]);
+        if (f != 0.f) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[i] = __builtin_fmaf(v[i], f, sum[i]);
+          l = __builtin_fmaf(lw, f, l);
+        }
+      }
+      *reinterpret_cast<f32x4*>(part_acc + static_cast<int64_t>(row) * kDim + 4 * piece) = sum;
+      if (piece == 0) part_ml[row] = f32x2{top, l};
+    }
+  }
+}
+
+struct SharedArgs {
+  const uint16_t* q;
+  const uint8_t* key_cache;
+  const uint8_t* value_cache;
+  const int32_t* tables;
+  const int4* plan;
+  float* part_acc;
+  f32x2* part_ml;
+  int64_t q_seq_stride, table_stride;
+  PlanShape shape;
+  int32_t block_size, block_shift, num_blocks, num_kv_heads, group, num_seqs, num_groups;
+  float scale_log2;
+};
+
+// Whether the plan was built for this batch.
+__device__ __forceinline__ bool plan_fits(const const_i32* plan, int32_t num_seqs, int32_t num_groups,
+                                          int32_t num_kv_heads, int32_t group) {
+  return plan[2] == num_seqs && plan[3] == num_groups && plan[4] == num_kv_heads && plan[5] == group;
+}
+
+template <bool kChunked, bool kHalf>
+__global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArgs a) {
+  __shared__ TileShared sh;
+  const const_i32* const plan = (const const_i32*)a.plan;
+  if (!plan_fits(plan, a.num_seqs, a.num_groups, a.num_kv_heads, a.group)) return;
+  const int32_t prefix_entries = min(static_cast<int64_t>(plan[0]), a.shape.prefix);
+  const int32_t rest_entries = min(static_cast<int64_t>(plan[1]), a.shape.rest);
+  const int32_t entry = static_cast<int32_t>(blockIdx.x / static_cast<uint32_t>(a.num_kv_heads));
+  const int32_t turn = static_cast<int32_t>(blockIdx.x) - entry * a.num_kv_heads;
+  if (entry >= prefix_entries + rest_entries) return;
+  // The kv head rotates with the entry, so that no XCD (workgroup id % 8)
+  // stays on one byte offset of the rows.
+  const int32_t period = 8 / min(8, a.num_kv_heads & -a.num_kv_heads);
+  const int32_t kh = (turn + entry / period) % a.num_kv_heads;
+  KeySource src;
+  src.k_head = a.key_cache + static_cast<int64_t>(kh) * (kDim * 2);
+  src.v_head = a.value_cache + static_cast<int64_t>(kh) * (kDim * 2);
+  src.zeros = reinterpret_cast<const uint8_t*>(a.plan + 2);
+  src.table_stride = a.table_stride;
+  src.row_bytes = static_cast<uint32_t>(a.num_kv_heads) * (kDim * 2);
+  src.block_size = a.block_size;
+  src.block_shift = a.block_shift;
+  src.num_blocks = a.num_blocks;
+  RowSource rows;
+  rows.q = a.q + static_cast<int64_t>(kh) * a.group * kDim;
+  rows.seq_stride = a.q_seq_stride;
+  rows.group = a.group;
+  if (entry < prefix_entries) {
+    const const_i32* const e = plan + 4 * (a.shape.prefix_at() + 2 * entry);
+    const int32_t log2 = e[3];
+    rows.first = e[0];
+    rows.row0 = e[1];
+    rows.rows = e[2];
+    src.begin = e[4];
+    src.end = e[5];
+    // Uniform exits for entries that name rows outside the batch.
+    if (rows.first < 0 || rows.row0 < 0 || rows.rows <= 0 || rows.rows > kEntryRows || src.begin < 0 ||
+        src.end <= src.begin ||
+        rows.first + (static_cast<int64_t>(rows.row0) + rows.rows - 1) / a.group >= a.num_seqs) {
+      return;
+    }
+    src.table = (const const_i32*)(a.tables + static_cast<int64_t>(rows.first) * a.table_stride);
+    const int64_t row = (static_cast<int64_t>(entry) * a.num_kv_heads + kh) * kEntryRows;
+    float* const acc = a.part_acc + row * kDim;
+    f32x2* const ml = a.part_ml + row;
+    if (log2 == 7) {
+      attend<4, 2, kChunked, kHalf>(sh, src, rows, a.scale_log2, acc, ml);
+    } else if (log2 == 6) {
+      attend<2, 2, kChunked, kHalf>(sh, src, rows, a.scale_log2, acc, ml);
+    } else if (log2 == 5) {
+      attend<1, 2, kChunked, kHalf>(sh, src, rows, a.scale_log2, acc, ml);
+    } else {
+      attend<1, 1, kChunked, kHalf>(sh, src, rows, a.scale_log2, acc, ml);
+    }
+    return;
+  }
+  const int32_t s = entry - prefix_entries;
+  const const_i32* const e = plan + 4 * (a.shape.rest_at() + s);
+  rows.first = e[0];
+  rows.row0 = 0;
+  rows.rows = a.group;
+  src.begin = e[1];
+  src.end = e[2];
+  if (rows.first < 0 || rows.first >= a.num_seqs || src.begin < 0 || src.end <= src.begin) return;
+  src.table = (const const_i32*)(a.tables + static_cast<int64_t>(rows.first) * a.table_stride);
+  const int64_t row = a.shape.prefix_rows(a.num_kv_heads) +
+                      (static_cast<int64_t>(s) * a.num_kv_heads + kh) * a.group;
+  attend<1, 1, kChunked, kHalf>(sh, src, rows, a.scale_log2, a.part_acc + row * kDim, a.part_ml + row);
+}
+
+// Adds up the partials of (sequence, query head) pairs: those of the prefix's
+// pieces, then the rest's.  kWaves wavefronts per pair, each every kWaves-th
+// batch; a lane holds two dims.
+constexpr int kMergeBatch = 8;
+template <bool kHalf, int kWaves>
+__global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a, uint16_t* __restrict__ out,
+                                                           int64_t out_seq_stride) {
+  constexpr int kPairs = 4 / kWaves;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int w4 = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int part_wave = w4 % kWaves;
+  const int64_t pair = static_cast<int64_t>(blockIdx.x) * kPairs + w4 / kWaves;
+  const int32_t num_q_heads = a.num_kv_heads * a.group;
+  const bool there = pair < static_cast<int64_t>(a.num_seqs) * num_q_heads;
+  if (kWaves == 1 && !there) return;  // (with more waves a workgroup is one pair)
+  const int32_t seq = static_cast<int32_t>(pair / num_q_heads);
+  const int32_t qh = static_cast<int32_t>(pair % num_q_heads);
+  const int32_t kh = qh / a.group, head = qh % a.group;
+  uint32_t* const dst = reinterpret_cast<uint32_t*>(out + seq * out_seq_stride + qh * kDim + 2 * lane);
+  const const_i32* const plan = (const const_i32*)a.plan;
+  if (!plan_fits(plan, a.num_seqs, a.num_groups, a.num_kv_heads, a.group)) {
+    // Another batch's plan: no partial was written.  NaN, not stale values.
+    if (part_wave == 0) *dst = kHalf ? 0x7E007E00u : 0x7FC07FC0u;
+    return;
+  }
+  const const_i32* const record = plan + 4 * (kPlanSeqs + 2 * static_cast<int64_t>(seq));
+  const int32_t rest_first = record[2], rest_count = record[3];
+  const int32_t pieces = record[5];
+  const int32_t row = record[6] * a.group + head;
+  const int32_t tile = row / kEntryRows;
+  const int64_t prefix_first = record[4] + static_cast<int64_t>(tile) * pieces;
+  const int64_t rest_row = a.shape.prefix_rows(a.num_kv_heads);
+  const int32_t parts = pieces + rest_count;
+  auto row_of = [&](int32_t p) -> int64_t {
+    if (p < pieces) {
+      const int64_t e = min(prefix_first + p, a.shape.prefix - 1);
+      return (e * a.num_kv_heads + kh) * kEntryRows + row % kEntryRows;
+    }
+    const int64_t e = min(static_cast<int64_t>(rest_first) + p - pieces, a.shape.rest - 1);
+    return rest_row + (e * a.num_kv_heads + kh) * a.group + head;
+  };
+  float run_max = -INFINITY, total = 0.f;
+  f32x2 sum = {0.f, 0.f};
+  for (int32_t p0 = part_wave * kMergeBatch; p0 < parts; p0 += kWaves * kMergeBatch) {
+    f32x2 ml[kMergeBatch], v[kMergeBatch];
+#pragma unroll
+    for (int i = 0; i < kMergeBatch; ++i) {
+      const int64_t at = row_of(min(p0 + i, parts - 1));
+      ml[i] = a.part_ml[at];
+      v[i] = *reinterpret_cast<const f32x2*>(a.part_acc + at * kDim + 2 * lane);
+    }
+    float top = run_max;
+#pragma unroll
+    for (int i = 0; i < kMergeBatch; ++i) {
+      if (p0 + i >= parts) ml[i] = f32x2{-INFINITY, 0.f};  // a repeat of the last one
+      top = fmaxf(top, ml[i].x);
+    }
+    const float keep = run_max == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(run_max - top);
+    sum *= keep;
+    total *= keep;
+#pragma unroll
+    for (int i = 0; i < kMergeBatch; ++i) {
+      if (ml[i].x == -INFINITY && ml[i].y == 0.f) continue;
+      const float f = ml[i].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml[i].x - top);
+      sum.x = __builtin_fmaf(v[i].x, f, sum.x);
+      sum.y = __builtin_fmaf(v[i].y, f, sum.y);
+      total = __builtin_fmaf(ml[i].y, f, total);
+    }
+    run_max = top;
+  }
+  if constexpr (kWaves > 1) {
+    __shared__ f32x2 s_sum[kWaves][kWave];
+    __shared__ f32x2 s_ml[kWaves];
+    s_sum[part_wave][lane] = sum;
+    if (lane == 0) s_ml[part_wave] = f32x2{run_max, total};
+    __syncthreads();
+    if (part_wave != 0) return;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) top = fmaxf(top, s_ml[w].x);
+    sum = f32x2{0.f, 0.f};
+    total = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const f32x2 ml = s_ml[w], v = s_sum[w][lane];
+      if (ml.x == -INFINITY && ml.y == 0.f) continue;
+      const float f = ml.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ml.x - top);
+      sum.x = __builtin_fmaf(v.x, f, sum.x);
+      sum.y = __builtin_fmaf(v.y, f, sum.y);
+      total = __builtin_fmaf(ml.y, f, total);
+    }
+  }
+  typedef typename Elem<kHalf>::T T;
+  const bool empty = total == 0.f;  // no key at all (a NaN sum is not empty)
+  const T x = static_cast<T>(empty ? 0.f : sum.x / total), y = static_cast<T>(empty ? 0.f : sum.y / total);
+  *dst = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, x)) |
+         (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, y)) << 16);
+}
+
+bool layout_ok(int64_t num_seqs, int64_t num_groups, int64_t num_kv_heads, int64_t num_q_heads) {
+  return num_seqs >= 0 && num_seqs <= NKV_MAX_PLAN_SEQS && num_groups >= 0 &&
+         num_groups <= NKV_MAX_PLAN_SEQS && num_kv_heads > 0 && num_kv_heads <= 4096 &&
+         num_q_heads > 0 && num_q_heads % num_kv_heads == 0 && num_q_heads / num_kv_heads <= kMaxGroup;
+}
+
+}  // namespace
+}  // namespace nkv
+
+extern "C" int64_t nkv_shared_plan_bytes(int64_t num_seqs, int64_t num_groups, int64_t num_kv_heads,
+                                         int64_t num_q_heads, int64_t rest_tokens) {
+  using namespace nkv;
+  if (!layout_ok(num_seqs, num_groups, num_kv_heads, num_q_heads)) return 0;
+  return 16 * plan_shape(num_seqs, num_groups, num_kv_heads, num_q_heads / num_kv_heads, rest_tokens).int4s();
+}
+
+extern "C" int64_t nkv_shared_workspace_bytes(int64_t num_seqs, int64_t num_groups, int64_t num_kv_heads,
+                                              int64_t num_q_heads, int64_t rest_tokens) {
+  using namespace nkv;
+  if (!layout_ok(num_seqs, num_groups, num_kv_heads, num_q_heads)) return 0;
+  const int64_t group = num_q_heads / num_kv_heads;
+  return plan_shape(num_seqs, num_groups, num_kv_heads, group, rest_tokens).rows(num_kv_heads, group) *
+         (kDim * 4 + 8);
+}
+
+extern "C" int nkv_build_shared_plan(const int32_t* cu_seqlens_k, int64_t num_seqs, const int32_t* cu_groups,
+                                     const int32_t* prefix_lens, int64_t num_groups, int64_t num_kv_heads,
+                                     int64_t num_q_heads, int64_t rest_tokens, void* plan,
+                                     int64_t plan_bytes, void* stream) {
+  using namespace nkv;
+  if (!layout_ok(num_seqs, num_groups, num_kv_heads, num_q_heads)) {
+    return nkv_fail(NKV_E_INVALID,
+                    "nkv_build_shared_plan: need at most %d sequences and groups, and at most %d query "
+                    "heads per kv head",
+                    NKV_MAX_PLAN_SEQS, kMaxGroup);
+  }
+  const int64_t group = num_q_heads / num_kv_heads;
+  const PlanShape shape = plan_shape(num_seqs, num_groups, num_kv_heads, group, rest_tokens);
+  if (plan_bytes != 16 * shape.int4s()) {
+    return nkv_fail(NKV_E_CAPACITY, "nkv_build_shared_plan: a plan of %lld bytes, exactly %lld are laid out",
+                    static_cast<long long>(plan_bytes), static_cast<long long>(16 * shape.int4s()));
+  }
+  if (!plan || !cu_seqlens_k || (num_groups > 0 && (!cu_groups || !prefix_lens))) {
+    return nkv_fail(NKV_E_INVALID, "nkv_build_shared_plan: null pointer");
+  }
+  if (reinterpret_cast<uint64_t>(plan) % 16 != 0) {
+    return nkv_fail(NKV_E_INVALID, "nkv_build_shared_plan: plan must be 16-byte aligned");
+  }
+  const GroupOf groups{cu_groups, prefix_lens, static_cast<int32_t>(num_groups), static_cast<int32_t>(num_seqs)};
+  const size_t lds = (static_cast<size_t>(std::max(num_seqs, num_groups)) + 1) * sizeof(int32_t);
+  shared_plan_kernel<<<dim3(1), dim3(kPlanThreads), lds, static_cast<hipStream_t>(stream)>>>(
+      cu_seqlens_k, groups, static_cast<int32_t>(num_kv_heads), static_cast<int32_t>(group), shape,
+      static_cast<int4*>(plan));
+  return nkv_check_launch("nkv_build_shared_plan");
+}
+
+extern "C" int nkv_shared_prefix_attention_decode(
+    const void* q, int64_t q_seq_stride, const void* key_cache, const void* value_cache,
+    const int32_t* block_tables, int64_t table_stride, const void* plan, int64_t plan_bytes,
+    int64_t num_seqs, int64_t num_groups, int64_t num_kv_heads, int64_t num_q_heads, int64_t head_dim,
+    int64_t block_size, int64_t num_blocks, int64_t rest_tokens, float scale, int32_t dtype,
+    void* workspace, int64_t workspace_bytes, void* out, int64_t out_seq_stride, void* stream) {
+  using namespace nkv;
+  const char* const what = "nkv_shared_prefix_attention_decode";
+  if (dtype != NKV_DTYPE_BFLOAT16 && dtype != NKV_DTYPE_FLOAT16) {
+    return nkv_fail(NKV_E_INVALID, "%s: only bfloat16 and float16 are supported", what);
+  }
+  if (head_dim != kDim) return nkv_fail(NKV_E_INVALID, "%s: head_dim must be %d", what, kDim);
+  if (!layout_ok(num_seqs, num_groups, num_kv_heads, num_q_heads)) {
+    return nkv_fail(NKV_E_INVALID,
+                    "%s: need at most %d sequences and groups, and 1 to %d query heads per kv head", what,
+                    NKV_MAX_PLAN_SEQS, kMaxGroup);
+  }
+  if (block_size <= 0 || num_blocks < 0 || num_blocks > INT32_MAX || block_size > INT32_MAX ||
+      num_blocks * block_size > INT32_MAX || table_stride < 0 || q_seq_stride < num_q_heads * head_dim ||
+      out_seq_stride < num_q_heads * head_dim) {
+    return nkv_fail(NKV_E_INVALID, "%s: bad sizes or strides", what);
+  }
+  // The chunk max is taken of the raw scores: it commutes with scale > 0 only.
+  if (!std::isfinite(scale) || !(scale > 0.f)) {
+    return nkv_fail(NKV_E_INVALID, "%s: scale must be finite and positive", what);
+  }
+  if (num_seqs == 0) return NKV_OK;
+  const int64_t group = num_q_heads / num_kv_heads;
+  const PlanShape shape = plan_shape(num_seqs, num_groups, num_kv_heads, group, rest_tokens);
+  if (plan_bytes != 16 * shape.int4s()) {
+    return nkv_fail(NKV_E_CAPACITY, "%s: a plan of %lld bytes, exactly %lld are laid out", what,
+                    static_cast<long long>(plan_bytes), static_cast<long long>(16 * shape.int4s()));
+  }
+  const int64_t rows = shape.rows(num_kv_heads, group);
+  if (workspace_bytes < rows * (kDim * 4 + 8)) {
+    return nkv_fail(NKV_E_CAPACITY, "%s: workspace of %lld bytes < %lld needed", what,
+                    static_cast<long long>(workspace_bytes), static_cast<long long>(rows * (kDim * 4 + 8)));
+  }
+  if (!q || !key_cache || !value_cache || !plan || !workspace || !out || (table_stride > 0 && !block_tables)) {
+    return nkv_fail(NKV_E_INVALID, "%s: null pointer", what);
+  }
+  if ((reinterpret_cast<uint64_t>(q) | reinterpret_cast<uint64_t>(key_cache) |
+       reinterpret_cast<uint64_t>(value_cache) | reinterpret_cast<uint64_t>(plan) |
+       reinterpret_cast<uint64_t>(workspace) | static_cast<uint64_t>(q_seq_stride * 2)) % 16 != 0 ||
+      (reinterpret_cast<uint64_t>(out) | static_cast<uint64_t>(out_seq_stride * 2)) % 4 != 0) {
+    return nkv_fail(NKV_E_INVALID,
+                    "%s: q/caches/plan/workspace must be 16-byte aligned and out rows 4-byte aligned", what);
+  }
+  const int64_t items = (shape.prefix + shape.rest) * num_kv_heads;
+  const int64_t pairs = num_seqs * num_q_heads;
+  if (items > INT32_MAX || pairs > INT32_MAX) {
+    return nkv_fail(NKV_E_INVALID, "%s: too many sequences and heads for one launch", what);
+  }
+  SharedArgs a;
+  a.q = static_cast<const uint16_t*>(q);
+  a.key_cache = static_cast<const uint8_t*>(key_cache);
+  a.value_cache = static_cast<const uint8_t*>(value_cache);
+  a.tables = block_tables;
+  a.plan = static_cast<const int4*>(plan);
+  a.part_acc = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<f32x2*>(a.part_acc + rows * kDim);
+  a.q_seq_stride = q_seq_stride;
+  a.table_stride = table_stride;
+  a.shape = shape;
+  a.block_size = static_cast<int32_t>(block_size);
+  a.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctzll(static_cast<uint64_t>(block_size)) : -1;
+  a.num_blocks = static_cast<int32_t>(num_blocks);
+  a.num_kv_heads = static_cast<int32_t>(num_kv_heads);
+  a.group = static_cast<int32_t>(group);
+  a.num_seqs = static_cast<int32_t>(num_seqs);
+  a.num_groups = static_cast<int32_t>(num_groups);
+  a.scale_log2 = scale * 1.4426950408889634f;  // log2(e)
+  const bool half = dtype == NKV_DTYPE_FLOAT16;
+  const bool chunked = block_size % kChunk == 0;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  void (*kernel)(SharedArgs) =
+      chunked ? (half ? shared_attention_kernel<true, true> : shared_attention_kernel<true, false>)
+              : (half ? shared_attention_kernel<false, true> : shared_attention_kernel<false, false>);
+  kernel<<<dim3(static_cast<unsigned>(items)), dim3(kThreads), 0, s>>>(a);
+  if (int rc = nkv_check_launch(what)) return rc;
+  const bool four = pairs <= 2048;
+  void (*merge)(SharedArgs, uint16_t*, int64_t) =
+      four ? (half ? shared_merge_kernel<true, 4> : shared_merge_kernel<false, 4>)
+           : (half ? shared_merge_kernel<true, 1> : shared_merge_kernel<false, 1>);
+  merge<<<dim3(static_cast<unsigned>(four ? pairs : (pairs + 3) / 4)), dim3(256), 0, s>>>(
+      a, static_cast<uint16_t*>(out), out_seq_stride);
+  return nkv_check_launch(what);
+}

@@ -192,6 +192,19 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
         ctypes.c_int, (c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr)),
     "nkv_rotary_table": (ctypes.c_int, (c_ptr, ctypes.c_double, c_i64, c_i64, c_ptr, c_ptr)),
     "nkv_rotary": (ctypes.c_int, (c_rotary, c_ptr)),
+    "nkv_shared_plan_bytes": (c_i64, (c_i64, c_i64, c_i64, c_i64, c_i64)),
+    "nkv_shared_workspace_bytes": (c_i64, (c_i64, c_i64, c_i64, c_i64, c_i64)),
+    "nkv_build_shared_plan": (
+        ctypes.c_int,
+        (c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr),
+    ),
+    "nkv_shared_prefix_attention_decode": (
+        ctypes.c_int,
+        (
+            c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64,
+            c_i64, c_i64, c_i64, c_i64, ctypes.c_float, c_i32, c_ptr, c_i64, c_ptr, c_i64, c_ptr,
+        ),
+    ),
     "nkv_pack_decode_pool": (
         ctypes.c_int,
         (c_pool, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_i64, c_ptr, c_ptr, c_ptr, c_ptr,

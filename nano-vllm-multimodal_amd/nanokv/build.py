@@ -32,6 +32,7 @@ SOURCES = (
     "nkv_store_gather.hip",
     "nkv_rotary.hip",
     "nkv_pages.hip",
+    "nkv_shared.hip",
 )
 OFFLOAD_ARCH = "gfx950"
 HIPCC_FLAGS = (

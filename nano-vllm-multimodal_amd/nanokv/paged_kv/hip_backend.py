@@ -59,6 +59,17 @@ class AttentionPlan(tuple):
         return self
 
 
+class SharedPrefixPlan:
+    """``plan`` of :meth:`HIPPagedKVBackend.build_shared_prefix_plan`, with
+    the counts it was built for: (sequences, groups, kv heads, query heads)
+    and the bound of the tokens that are not shared."""
+
+    def __init__(self, plan: torch.Tensor, counts: tuple[int, int, int, int], rest_tokens: int) -> None:
+        self.plan = plan
+        self.counts = counts
+        self.rest_tokens = rest_tokens
+
+
 def reset_hip_backend_state_for_tests() -> None:
     global _READY
     with _LOAD_LOCK:
@@ -453,6 +464,76 @@ class HIPPagedKVBackend:
                                     cu_seqlens_k, plan, float(softmax_scale), out)
         return out
 
+    # ------------------------------------- decode over shared prefixes
+    def build_shared_prefix_plan(
+        self,
+        cache: torch.Tensor,
+        cu_seqlens_k: torch.Tensor,
+        total_tokens: int,
+        cu_groups: torch.Tensor,
+        prefix_lens: torch.Tensor,
+        num_q_heads: int,
+        *,
+        suffix_tokens: int | None = None,
+    ) -> SharedPrefixPlan:
+        """Plan of :meth:`shared_prefix_attention_decode` for one step (all of
+        its layers): it depends on the context lengths, the groups and the
+        head counts.  ``suffix_tokens``, the sum of the contexts' rows past
+        their shared prefixes where the caller knows it, bounds the launch
+        and the workspace; otherwise ``total_tokens`` does.  (Either may
+        understate the sum: the contexts are served all the same.)"""
+        self._load()
+        validate_groups(cu_seqlens_k, cu_groups, prefix_lens)
+        rest = int(total_tokens) if suffix_tokens is None else int(suffix_tokens)
+        if rest < 0:
+            raise ValueError("total_tokens and suffix_tokens must be non-negative")
+        kv_heads, q_heads = int(cache.shape[2]), int(num_q_heads)
+        plan = ops.build_shared_prefix_plan(cu_seqlens_k, cu_groups, prefix_lens, kv_heads, q_heads, rest)
+        counts = (cu_seqlens_k.numel() - 1, cu_groups.numel() - 1, kv_heads, q_heads)
+        return SharedPrefixPlan(plan, counts, rest)
+
+    def shared_prefix_attention_decode(
+        self,
+        q: torch.Tensor,
+        key_cache: torch.Tensor,
+        value_cache: torch.Tensor,
+        block_tables: torch.Tensor,
+        cu_seqlens_k: torch.Tensor,
+        total_tokens: int,
+        cu_groups: torch.Tensor,
+        prefix_lens: torch.Tensor,
+        softmax_scale: float,
+        *,
+        plan: SharedPrefixPlan | None = None,
+        out: torch.Tensor | None = None,
+    ) -> torch.Tensor:
+        """:meth:`paged_attention_decode` for a batch whose sequences share
+        prefixes, each prefix read once for its whole group.  Group g is the
+        sequences [cu_groups[g], cu_groups[g+1]) of the batch; the first
+        prefix_lens[g] rows of their contexts are the same (shared blocks, or
+        copies of a block, as a fork leaves them) and are read through the
+        table of the group's first sequence.  Sequences alone in a group, in
+        no group or shorter than its prefix are read through their own
+        tables.  ``plan`` from :meth:`build_shared_prefix_plan`, one per
+        step, serves every layer."""
+        validate_varlen_inputs(key_cache, value_cache, block_tables, cu_seqlens_k, total_tokens)
+        if q.ndim != 3 or q.shape[0] != block_tables.shape[0]:
+            raise ValueError("q must be [num_seqs, num_q_heads, head_dim] with one row per sequence")
+        if not _READY:
+            self._load()
+        if plan is None:
+            plan = self.build_shared_prefix_plan(key_cache, cu_seqlens_k, total_tokens, cu_groups,
+                                                 prefix_lens, q.shape[1])
+        here = (q.shape[0], cu_groups.numel() - 1, key_cache.shape[2], q.shape[1])
+        if plan.counts != here:
+            raise ValueError(f"shared-prefix plan was built for {plan.counts} (sequences, groups, kv heads, "
+                             f"query heads), not {here}: build it for this batch and cache")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ops.shared_prefix_attention_decode(q, key_cache, value_cache, block_tables, plan.plan, here[1],
+                                           plan.rest_tokens, float(softmax_scale), out)
+        return out
+
     # ------------------------------------------------- rotary positions
     def rotary(
         self,
@@ -541,6 +622,16 @@ class HIPPagedKVBackend:
         if not pairs.is_cuda:
             pairs = pairs.to(device=cache.device, dtype=torch.int32)
         ops.copy_blocks(cache, target, pairs)
+
+
+def validate_groups(cu_seqlens_k: torch.Tensor, cu_groups: torch.Tensor, prefix_lens: torch.Tensor) -> None:
+    """Group values, when index validation is enabled (it synchronises)."""
+    if cu_groups.numel() and index_value_validation_enabled(cu_groups):
+        cu, prefix = cu_groups.cpu(), prefix_lens.cpu()
+        if bool((cu < 0).any()) or bool((cu[1:] < cu[:-1]).any()) or int(cu[-1]) >= cu_seqlens_k.numel():
+            raise ValueError("cu_groups must be non-decreasing, from 0 to at most the number of sequences")
+        if bool((prefix < 0).any()):
+            raise ValueError("prefix_lens must be non-negative")
 
 
 def validate_positions(positions: torch.Tensor, table) -> None:

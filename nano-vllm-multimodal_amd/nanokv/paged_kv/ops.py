@@ -40,6 +40,14 @@ too, paged_kv_cuda.cu:168-171).  Additive ops, with no reference schema:
                  Tensor table, int layout, int[] section_ends,
                  Tensor(c!) q_out, Tensor(d!)? k_out=None) -> ()
     copy_blocks(Tensor cache, Tensor(a!) dst, Tensor pairs) -> ()
+    build_shared_prefix_plan(Tensor cu_seqlens_k, Tensor cu_groups,
+                             Tensor prefix_lens, int num_kv_heads,
+                             int num_q_heads, int rest_tokens) -> Tensor
+    shared_prefix_attention_decode(Tensor q, Tensor key_cache,
+                                   Tensor value_cache, Tensor block_tables,
+                                   Tensor plan, int num_groups,
+                                   int rest_tokens, float scale,
+                                   Tensor(a!) out) -> ()
 
 Every kernel runs on the current stream of the tensors' device and returns
 before it completes, like the reference ops.
@@ -89,6 +97,11 @@ SCHEMAS = {
     "Tensor(b!) value_cache, Tensor slot_mapping, Tensor positions, Tensor table, int layout, "
     "int[] section_ends, Tensor(c!) q_out, Tensor(d!)? k_out=None) -> ()",
     "copy_blocks": "copy_blocks(Tensor cache, Tensor(a!) dst, Tensor pairs) -> ()",
+    "build_shared_prefix_plan": "build_shared_prefix_plan(Tensor cu_seqlens_k, Tensor cu_groups, "
+    "Tensor prefix_lens, int num_kv_heads, int num_q_heads, int rest_tokens) -> Tensor",
+    "shared_prefix_attention_decode": "shared_prefix_attention_decode(Tensor q, Tensor key_cache, "
+    "Tensor value_cache, Tensor block_tables, Tensor plan, int num_groups, int rest_tokens, "
+    "float scale, Tensor(a!) out) -> ()",
 }
 
 DTYPE_CODES = {
@@ -689,6 +702,66 @@ def _copy_blocks_impl(cache, dst, pairs) -> None:
     _lib.check(status, "nanovllm_paged_kv::copy_blocks")
 
 
+def _build_shared_prefix_plan_impl(cu_seqlens_k, cu_groups, prefix_lens, num_kv_heads: int,
+                                   num_q_heads: int, rest_tokens: int) -> torch.Tensor:
+    device = _require_device("paged KV HIP shared-prefix plan", cu_seqlens_k, cu_groups, prefix_lens)
+    num_seqs = _require_cu("cu_seqlens_k", cu_seqlens_k)
+    num_groups = _require_cu("cu_groups", cu_groups)
+    if prefix_lens.dtype != torch.int32 or prefix_lens.shape != (num_groups,) or not prefix_lens.is_contiguous():
+        raise ValueError("prefix_lens must be a contiguous 1-D int32 tensor with one entry per group")
+    library = _lib.load_library()
+    nbytes = int(library.nkv_shared_plan_bytes(num_seqs, num_groups, num_kv_heads, num_q_heads, rest_tokens))
+    if nbytes == 0:
+        raise ValueError(f"shared-prefix attention supports at most {_lib.NKV_MAX_PLAN_SEQS} sequences "
+                         "and 1 to 16 query heads per kv head")
+    plan = torch.empty(nbytes // 4, dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        status = library.nkv_build_shared_plan(
+            cu_seqlens_k.data_ptr(), num_seqs, cu_groups.data_ptr(),
+            prefix_lens.data_ptr() if num_groups else None, num_groups, num_kv_heads, num_q_heads,
+            rest_tokens, plan.data_ptr(), nbytes, _stream(device))
+    _lib.check(status, "nanovllm_paged_kv::build_shared_prefix_plan")
+    return plan
+
+
+def _shared_prefix_decode_impl(q, key_cache, value_cache, block_tables, plan, num_groups: int,
+                               rest_tokens: int, scale: float, out) -> None:
+    device = _require_device("shared-prefix attention", q, key_cache, value_cache, block_tables, plan, out)
+    if (block_tables.dtype != torch.int32 or block_tables.ndim != 2
+            or block_tables.shape[0] != q.shape[0] or not block_tables.is_contiguous()):
+        raise ValueError("block_tables must be a contiguous [num_seqs, width] int32 tensor")
+    _require_contiguous_cache("shared-prefix attention", key_cache, value_cache)
+    if key_cache.ndim != 4 or key_cache.shape != value_cache.shape:
+        raise ValueError("key and value cache shape must match [blocks, block, kv_heads, head_dim]")
+    _require_attention_dtype("shared-prefix attention", q, key_cache, value_cache, out)
+    if q.ndim != 3 or q.stride(2) != 1 or q.stride(1) != q.shape[2]:
+        raise ValueError("q must be [num_seqs, num_q_heads, head_dim] with contiguous heads")
+    if out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != out.shape[2]:
+        raise ValueError("out must match q's shape with contiguous heads")
+    num_blocks, block_size, num_kv_heads, head_dim = key_cache.shape
+    if q.shape[2] != head_dim:
+        raise ValueError("q head_dim does not match the cache")
+    if plan.dtype != torch.int32 or plan.ndim != 1 or not plan.is_contiguous():
+        raise ValueError("shared-prefix plan must be a contiguous 1-D int32 tensor")
+    num_seqs, num_q_heads = q.shape[0], q.shape[1]
+    # Rows of a batch of one may have any stride: nothing steps over them.
+    row = num_q_heads * head_dim
+    q_stride = q.stride(0) if num_seqs > 1 else row
+    out_stride = out.stride(0) if num_seqs > 1 else row
+    library = _lib.load_library()
+    nbytes = int(library.nkv_shared_workspace_bytes(num_seqs, num_groups, num_kv_heads, num_q_heads,
+                                                    rest_tokens))
+    workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=device)
+    with torch.cuda.device(device):
+        status = library.nkv_shared_prefix_attention_decode(
+            q.data_ptr(), q_stride, key_cache.data_ptr(), value_cache.data_ptr(),
+            block_tables.data_ptr(), block_tables.shape[1], plan.data_ptr(), plan.numel() * 4, num_seqs,
+            num_groups, num_kv_heads, num_q_heads, head_dim, block_size, num_blocks, rest_tokens,
+            float(scale), DTYPE_CODES[q.dtype], workspace.data_ptr(), nbytes, out.data_ptr(),
+            out_stride, _stream(device))
+    _lib.check(status, "nanovllm_paged_kv::shared_prefix_attention_decode")
+
+
 def register_ops() -> None:
     """Define the schemas (unless another library already did) and register
     the HIP implementations on the CUDA key.  Idempotent."""
@@ -715,6 +788,8 @@ def register_ops() -> None:
         fragment.impl("rotary", _rotary_impl, "CUDA")
         fragment.impl("rotary_store", _rotary_store_impl, "CUDA")
         fragment.impl("copy_blocks", _copy_blocks_impl, "CUDA")
+        fragment.impl("build_shared_prefix_plan", _build_shared_prefix_plan_impl, "CUDA")
+        fragment.impl("shared_prefix_attention_decode", _shared_prefix_decode_impl, "CUDA")
         _FRAGMENT = fragment
 
 
@@ -735,3 +810,5 @@ store_gather = _store_gather_impl
 rotary = _rotary_impl
 rotary_store = _rotary_store_impl
 copy_blocks = _copy_blocks_impl
+build_shared_prefix_plan = _build_shared_prefix_plan_impl
+shared_prefix_attention_decode = _shared_prefix_decode_impl

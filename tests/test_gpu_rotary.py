@@ -11,6 +11,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from nanokv.packing import capture_graph
 from nanokv.rotary import RotaryTable
 
 pytestmark = pytest.mark.gpu
@@ -184,7 +185,7 @@ def test_no_tokens_other_streams_and_graphs(backend, gpu_device):
     # Captured: new values in the same buffers, several replays.
     q2, k2, p2 = q.clone(), k.clone(), positions.clone()
     graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
+    with capture_graph(graph):
         captured = backend.rotary_store(q2, k2, v, kc, vc, slots, p2, table)
     for step in range(3):
         p2.copy_((positions + 11 * step) % 256)
