@@ -1,4 +1,5 @@
-// Per-call host path of the hip backend's store, gather and attention.
+// Per-call host path of the hip backend's store, gather, attention, rotary
+// positions and block copies.
 //
 // The reference's SDPA decode calls its backend's gather twice per request
 // per layer (nanovllm/layers/attention.py:284-300) and its store once per
@@ -404,6 +405,197 @@ py::object varlen(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
   });
 }
 
+// ------------------------------ rotary positions, block copies, shared prefixes
+//
+// As the attention calls: whole when every tensor is as the kernels take it,
+// None where the Python path has to look.  (The caller has made sure that the
+// stream's device is the current one.)
+using RotaryFn = decltype(&nkv_rotary);
+using CopyBlocksFn = decltype(&nkv_copy_blocks);
+using SharedWorkspaceFn = decltype(&nkv_shared_workspace_bytes);
+using SharedFn = decltype(&nkv_shared_prefix_attention_decode);
+
+RotaryFn g_rotary = nullptr;
+CopyBlocksFn g_copy_blocks = nullptr;
+SharedWorkspaceFn g_shared_workspace = nullptr;
+SharedFn g_shared = nullptr;
+
+bool kv_type(at::ScalarType type) { return half_type(type) || type == at::kFloat; }
+// [tokens, heads, head_dim] with a contiguous head_dim.
+bool heads_of(const at::Tensor& t, int64_t tokens, int64_t dim, at::ScalarType type,
+              const at::Device& device) {
+  return t.dim() == 3 && t.scalar_type() == type && on(t, device) && t.size(0) == tokens &&
+         t.size(2) == dim && t.stride(2) == 1;
+}
+bool head_output(const at::Tensor& out, const at::Tensor& like) {
+  return out.sizes() == like.sizes() &&
+         heads_of(out, like.size(0), like.size(2), like.scalar_type(), like.device());
+}
+
+// Rotated q and k, or, with the caches, q rotated and k and v stored; k_out
+// is then optional.  Returns q_out, or (q_out, k_out) without caches.
+py::object rotary(const at::Tensor& q, const at::Tensor& k, const c10::optional<at::Tensor>& v,
+                  const c10::optional<at::Tensor>& key_cache, const c10::optional<at::Tensor>& value_cache,
+                  const c10::optional<at::Tensor>& slots, const at::Tensor& positions,
+                  const at::Tensor& table, int64_t layout, int64_t end0, int64_t end1,
+                  const c10::optional<at::Tensor>& q_out_in, const c10::optional<at::Tensor>& k_out_in,
+                  int64_t stream) {
+  const at::Device device = q.device();
+  const at::ScalarType type = q.scalar_type();
+  if (g_rotary == nullptr || !q.is_cuda() || !kv_type(type) || q.dim() != 3 || q.size(0) == 0 ||
+      q.size(2) == 0) {
+    return py::none();
+  }
+  const int64_t tokens = q.size(0), dim = q.size(2);
+  const bool store = key_cache.has_value();
+  if (!heads_of(q, tokens, dim, type, device) || !heads_of(k, tokens, dim, type, device) ||
+      (q_out_in.has_value() && !head_output(*q_out_in, q)) ||
+      (k_out_in.has_value() && !head_output(*k_out_in, k)) || !on(table, device) || table.dim() != 3 ||
+      table.size(2) != 2 || table.scalar_type() != at::kFloat || !table.is_contiguous() ||
+      table.size(0) == 0 || table.size(1) == 0 || 2 * table.size(1) > dim || !on(positions, device) ||
+      (positions.scalar_type() != at::kInt && positions.scalar_type() != at::kLong) ||
+      index_values_checked(positions)) {
+    return py::none();
+  }
+  int64_t row_stride = 0;
+  if (positions.dim() == 2) {
+    row_stride = positions.stride(0);
+    if (positions.size(0) != 3 || positions.size(1) != tokens || row_stride < tokens ||
+        (end0 == table.size(1) && end1 == table.size(1))) {
+      return py::none();
+    }
+  } else if (positions.dim() != 1 || positions.size(0) != tokens) {
+    return py::none();
+  }
+  if (tokens > 1 && positions.stride(-1) != 1) return py::none();
+  nkv_rotary_desc d{};
+  if (store) {
+    const at::Tensor &kc = *key_cache, &vc = *value_cache, &sl = *slots;
+    if (!heads_of(*v, tokens, dim, type, device) || v->sizes() != k.sizes() || kc.dim() != 4 ||
+        kc.sizes() != vc.sizes() || kc.scalar_type() != type || vc.scalar_type() != type ||
+        !on(kc, device) || !on(vc, device) || !kc.is_contiguous() || !vc.is_contiguous() ||
+        kc.size(2) != k.size(1) || kc.size(3) != dim || !int32_vector(sl, device) ||
+        sl.size(0) != tokens || kc.numel() == 0) {
+      return py::none();
+    }
+    d.v = v->data_ptr();
+    d.v_token_stride = v->stride(0);
+    d.v_head_stride = v->stride(1);
+    d.key_cache = kc.data_ptr();
+    d.value_cache = vc.data_ptr();
+    d.slot_mapping = sl.data_ptr<int32_t>();
+    d.num_slots = kc.size(0) * kc.size(1);
+  }
+  at::Tensor q_out, k_out;
+  {
+    py::gil_scoped_release unlocked;
+    q_out = q_out_in.has_value() ? *q_out_in : at::empty(q.sizes(), q.options());
+    if (k_out_in.has_value()) {
+      k_out = *k_out_in;
+    } else if (!store) {
+      k_out = at::empty(k.sizes(), k.options());
+    }
+    d.q = q.data_ptr();
+    d.k = k.data_ptr();
+    d.q_out = q_out.data_ptr();
+    d.q_token_stride = q.stride(0);
+    d.q_head_stride = q.stride(1);
+    d.k_token_stride = k.stride(0);
+    d.k_head_stride = k.stride(1);
+    d.q_out_token_stride = q_out.stride(0);
+    d.q_out_head_stride = q_out.stride(1);
+    if (k_out.defined()) {
+      d.k_out = k_out.data_ptr();
+      d.k_out_token_stride = k_out.stride(0);
+      d.k_out_head_stride = k_out.stride(1);
+    }
+    d.positions = positions.data_ptr();
+    d.position_bytes = static_cast<int32_t>(positions.element_size());
+    d.position_row_stride = row_stride;
+    d.section_ends[0] = end0;
+    d.section_ends[1] = end1;
+    d.table = table.data_ptr<float>();
+    d.max_position = table.size(0);
+    d.rotary_dim = 2 * table.size(1);
+    d.num_tokens = tokens;
+    d.num_q_heads = q.size(1);
+    d.num_kv_heads = k.size(1);
+    d.head_dim = dim;
+    d.layout = static_cast<int32_t>(layout);
+    d.dtype = dtype_code(type);
+    check_status(g_rotary(&d, reinterpret_cast<void*>(stream)), "nanovllm_paged_kv::rotary");
+  }
+  if (store) return py::cast(q_out);
+  return py::make_tuple(q_out, k_out);
+}
+
+// Pairs on the device; true when the launch was made.
+bool copy_blocks(const at::Tensor& cache, const at::Tensor& dst, const at::Tensor& pairs, int64_t stream) {
+  const at::Device device = cache.device();
+  const int64_t dims = cache.dim();
+  if (g_copy_blocks == nullptr || !cache.is_cuda() || dims < 4 || dst.dim() != dims ||
+      !kv_type(cache.scalar_type()) || dst.scalar_type() != cache.scalar_type() || !on(dst, device) ||
+      !cache.is_contiguous() || !dst.is_contiguous() || !int32_matrix(pairs, device) ||
+      pairs.size(1) != 2 || pairs.size(0) == 0 || cache.numel() == 0 || dst.numel() == 0 ||
+      index_values_checked(pairs)) {
+    return false;
+  }
+  int64_t planes = 1, block = cache.element_size();
+  for (int64_t i = 0; i < dims; ++i) {
+    if (i == dims - 4) continue;
+    if (cache.size(i) != dst.size(i)) return false;
+    (i < dims - 4 ? planes : block) *= cache.size(i);
+  }
+  const auto a = reinterpret_cast<uintptr_t>(cache.data_ptr()), b = reinterpret_cast<uintptr_t>(dst.data_ptr());
+  const bool same = a == b && cache.size(dims - 4) == dst.size(dims - 4);
+  if (!same && a < b + static_cast<uintptr_t>(dst.nbytes()) && b < a + static_cast<uintptr_t>(cache.nbytes())) {
+    return false;
+  }
+  py::gil_scoped_release unlocked;
+  check_status(g_copy_blocks(cache.data_ptr(), dst.data_ptr(), planes, cache.size(dims - 4),
+                             dst.size(dims - 4), block, pairs.data_ptr<int32_t>(), pairs.size(0),
+                             reinterpret_cast<void*>(stream)),
+               "nanovllm_paged_kv::copy_blocks");
+  return true;
+}
+
+// Decode over shared prefixes with a plan built for these counts.
+py::object shared_decode(const at::Tensor& q, const at::Tensor& key_cache, const at::Tensor& value_cache,
+                         const at::Tensor& tables, const at::Tensor& cu_seqlens_k, int64_t total_tokens,
+                         const at::Tensor& plan, int64_t num_groups, int64_t rest_tokens, double scale,
+                         const c10::optional<at::Tensor>& out_in, int64_t stream) {
+  const at::Device device = q.device();
+  const at::ScalarType type = q.scalar_type();
+  if (g_shared == nullptr || !q.is_cuda() || !half_type(type) || !head_rows(q, type, device) ||
+      !caches(key_cache, value_cache, type, device) || !int32_matrix(tables, device) ||
+      !int32_vector(plan, device) || !int32_vector(cu_seqlens_k, device) || total_tokens < 0 ||
+      q.size(0) < 2 || tables.size(0) != q.size(0) || cu_seqlens_k.size(0) != q.size(0) + 1 ||
+      index_values_checked(tables)) {
+    return py::none();
+  }
+  return run_unlocked([&]() -> at::Tensor {
+    const at::Tensor out = output_for(q, out_in);
+    if (!out.defined()) return {};
+    const int64_t need = g_shared_workspace(q.size(0), num_groups, key_cache.size(2), q.size(1), rest_tokens);
+    const at::Tensor workspace = bytes_on(std::max<int64_t>(need, 16), q);
+    check_status(g_shared(q.data_ptr(), q.stride(0), key_cache.data_ptr(), value_cache.data_ptr(),
+                          tables.data_ptr<int32_t>(), tables.size(1), plan.data_ptr(), plan.size(0) * 4,
+                          q.size(0), num_groups, key_cache.size(2), q.size(1), kDim, key_cache.size(1),
+                          key_cache.size(0), rest_tokens, static_cast<float>(scale), dtype_code(type),
+                          workspace.data_ptr(), need, out.data_ptr(), out.stride(0),
+                          reinterpret_cast<void*>(stream)),
+                 "nanovllm_paged_kv::shared_prefix_attention_decode");
+    return out;
+  });
+}
+
+void bind_operators(uintptr_t rotary_fn, uintptr_t copy_fn, uintptr_t workspace_fn, uintptr_t shared_fn) {
+  g_rotary = reinterpret_cast<RotaryFn>(rotary_fn);
+  g_copy_blocks = reinterpret_cast<CopyBlocksFn>(copy_fn);
+  g_shared_workspace = reinterpret_cast<SharedWorkspaceFn>(workspace_fn);
+  g_shared = reinterpret_cast<SharedFn>(shared_fn);
+}
+
 void bind_attention(uintptr_t decode_capacity, uintptr_t decode_workspace, uintptr_t decode_fn,
                     uintptr_t prefill_capacity, uintptr_t prefill_plan_fn, uintptr_t prefill_workspace,
                     uintptr_t prefill_fn, uintptr_t varlen_fn) {
@@ -433,6 +625,14 @@ PYBIND11_MODULE(_nkv_host, m) {
   m.def("prefill", &prefill, "paged prefill attention; None when the general path has to look at it");
   m.def("varlen", &varlen, "prefill attention over keys back to back; None when the general path "
                            "has to look at it");
+  m.def("bind_operators", &bind_operators,
+        "set the library's rotary, block copy and shared-prefix entry points");
+  m.def("rotary", &rotary, "rotary positions, with or without the store; None when the general path "
+                           "has to look at it");
+  m.def("copy_blocks", &copy_blocks, "block copy by pairs on the device; false when the general path "
+                                     "has to look at it");
+  m.def("shared_decode", &shared_decode, "planned decode attention over shared prefixes; None when the "
+                                         "general path has to look at it");
   m.def("store", &store, "validated store launch on a stream");
   m.def("gather", &gather, "validated gather launch on a stream; returns the new tensor");
   m.def("check_store", &check_store, "the store validator's checks (no launch)");

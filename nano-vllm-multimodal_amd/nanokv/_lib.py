@@ -319,6 +319,10 @@ HOST_ATTENTION_ENTRIES = (
     "nkv_prefill_plan_capacity", "nkv_build_prefill_plan", "nkv_prefill_workspace_bytes",
     "nkv_paged_attention_prefill_split", "nkv_varlen_attention_prefill",
 )
+# The rest of the host binding, in bind_operators' order.
+HOST_OPERATOR_ENTRIES = (
+    "nkv_rotary", "nkv_copy_blocks", "nkv_shared_workspace_bytes", "nkv_shared_prefix_attention_decode",
+)
 
 
 def load_host():
@@ -354,6 +358,7 @@ def load_host():
 
             module.bind(address("nkv_store"), address("nkv_gather"), address("nkv_last_error"))
             module.bind_attention(*map(address, HOST_ATTENTION_ENTRIES))
+            module.bind_operators(*map(address, HOST_OPERATOR_ENTRIES))
             _HOST = module
     return _HOST
 

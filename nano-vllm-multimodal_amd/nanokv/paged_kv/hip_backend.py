@@ -516,6 +516,18 @@ class HIPPagedKVBackend:
         no group or shorter than its prefix are read through their own
         tables.  ``plan`` from :meth:`build_shared_prefix_plan`, one per
         step, serves every layer."""
+        # A planned call with everything as the kernels take it runs in the
+        # host binding (csrc/nkv_host.cpp); None: the checks below decide.
+        if plan is not None and q.ndim == 3 and plan.counts == (
+                q.shape[0], cu_groups.shape[0] - 1, key_cache.shape[2], q.shape[1]):
+            index = q.get_device()
+            if ops.is_current_device(index):
+                done = _HOST.shared_decode(q, key_cache, value_cache, block_tables, cu_seqlens_k,
+                                           int(total_tokens), plan.plan, plan.counts[1],
+                                           plan.rest_tokens, float(softmax_scale), out,
+                                           ops.stream_of(index))
+                if done is not None:
+                    return done if out is None else out
         validate_varlen_inputs(key_cache, value_cache, block_tables, cu_seqlens_k, total_tokens)
         if q.ndim != 3 or q.shape[0] != block_tables.shape[0]:
             raise ValueError("q must be [num_seqs, num_q_heads, head_dim] with one row per sequence")
@@ -552,6 +564,14 @@ class HIPPagedKVBackend:
         whose position is outside the table gets zeros."""
         if not _READY:
             self._load()
+        index = q.get_device()
+        if ops.is_current_device(index):
+            ends = table.section_ends
+            q_out, k_out = (None, None) if out is None else out
+            done = _HOST.rotary(q, k, None, None, None, None, positions, table.table, table.layout_code,
+                                ends[0], ends[1], q_out, k_out, ops.stream_of(index))
+            if done is not None:
+                return done if out is None else out
         validate_positions(positions, table)
         if out is None:
             out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
@@ -581,6 +601,13 @@ class HIPPagedKVBackend:
         stored."""
         if not _READY:
             self._load()
+        index = q.get_device()
+        if ops.is_current_device(index):
+            ends = table.section_ends
+            done = _HOST.rotary(q, k, v, key_cache, value_cache, slot_mapping, positions, table.table,
+                                table.layout_code, ends[0], ends[1], q_out, k_out, ops.stream_of(index))
+            if done is not None:
+                return done if q_out is None else q_out
         validate_store_inputs(k, v, key_cache, value_cache, slot_mapping)
         validate_positions(positions, table)
         if q_out is None:
@@ -610,7 +637,11 @@ class HIPPagedKVBackend:
         if not _READY:
             self._load()
         target = cache if dst is None else dst
-        if not isinstance(pairs, torch.Tensor):
+        if isinstance(pairs, torch.Tensor):
+            index = cache.get_device()
+            if ops.is_current_device(index) and _HOST.copy_blocks(cache, target, pairs, ops.stream_of(index)):
+                return
+        else:
             pairs = torch.tensor([tuple(p) for p in pairs], dtype=torch.int32).reshape(-1, 2)
         if pairs.ndim != 2 or pairs.shape[1] != 2 or pairs.dtype not in (torch.int32, torch.int64):
             raise ValueError("block copy: pairs must be [n, 2] int32")

@@ -139,6 +139,17 @@ def current_stream_handle(device: torch.device) -> int:
 _stream = current_stream_handle
 
 
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None)
+
+
+def is_current_device(index: int) -> bool:
+    """Whether GPU ``index`` is the calling thread's current device.  The
+    default stream's handle is 0 on every GPU: a launch on it runs on the
+    current one."""
+    return index >= 0 and index == (_CURRENT_DEVICE() if _CURRENT_DEVICE is not None
+                                    else torch.cuda.current_device())
+
+
 def _require_device(what: str, *tensors: torch.Tensor) -> torch.device:
     index = tensors[0].get_device()  # -1 for host tensors
     for tensor in tensors:
