@@ -41,13 +41,28 @@ constexpr int kDim = 128;
 constexpr int kThreads = 256;
 constexpr int kTileKeys = 64;
 constexpr int kChunk = 16;        // keys a wavefront copies per tile
+constexpr uint32_t kTileBytes = kTileKeys * 256;
 constexpr int kMaxGroup = 16;     // query heads per kv head
-constexpr int kEntryRows = 128;   // partial rows kept per prefix entry and kv head
+constexpr int kTileRows = 128;    // query rows of a prefix tile at most
+constexpr int kMinTileRows = 32;  // ... and at least, where a group has more
+#ifndef NKV_SHARED_TILE_LOG2
+#define NKV_SHARED_TILE_LOG2 7
+#endif
 constexpr int kPlanThreads = 1024;
 constexpr int kSlots = 512;       // workgroups resident on the chip: two per CU
-constexpr int kRestRounds = 4;    // entries of the rests: at most so many rounds of workgroups
-constexpr int kMinPrefixTiles = 2;
-constexpr int kMinRestTiles = 2;
+#ifndef NKV_SHARED_REST_ROUNDS
+#define NKV_SHARED_REST_ROUNDS 4  // entries of the rests: about so many rounds of workgroups
+#endif
+#ifndef NKV_SHARED_MIN_PREFIX
+#define NKV_SHARED_MIN_PREFIX 2  // shortest piece of a prefix, in 64-key tiles
+#endif
+#ifndef NKV_SHARED_MIN_REST
+#define NKV_SHARED_MIN_REST 2  // shortest entry of a rest
+#endif
+constexpr int kRestRounds = NKV_SHARED_REST_ROUNDS;
+constexpr int kMinPrefixTiles = NKV_SHARED_MIN_PREFIX;
+constexpr int kMinRestTiles = NKV_SHARED_MIN_REST;
+constexpr int32_t kMaxLength = 0x7FFFFF00;
 constexpr float kRescaleLog2 = 8.f;  // the reference max moves only past this
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -60,32 +75,37 @@ typedef __attribute__((address_space(4))) const int32_t const_i32;
 //   [1]  {num_kv_heads, query heads per kv head, 0, 0}
 //   [2, 18)  256 bytes of zeros, the row that dropped keys copy
 //   two per sequence  {rest's first row, context length, first rest entry, rest entries}
-//                     {first entry of its group's first tile, pieces per tile, member, log2 tile rows}
-//   two per prefix entry  {first sequence, first query row, query rows, log2 tile rows}
-//                         {first key, past the last, 0, 0}
+//                     {first entry of its group's first tile, pieces per tile, member, rows per tile}
+//   two per prefix entry  {first sequence, first query row, query rows, log2 of the rows its form holds}
+//                         {first key, past the last, rows per tile, whether the group has one tile}
 //   one per rest entry  {sequence, first row, past the last, 0}
+// Entries past the last of their kind are empty, so that a workgroup finds
+// its own at a fixed place, without the counts.
 // The query rows of a group and kv head are member-major, (member, head).
 constexpr int kPlanSeqs = 18;
 struct PlanShape {
   int64_t seqs, prefix, rest;  // sequences and entries to allocate
+  int64_t prefix_rows;         // partial rows of the prefix entries, per kv head
   __host__ __device__ int64_t prefix_at() const { return kPlanSeqs + 2 * seqs; }
   __host__ __device__ int64_t rest_at() const { return prefix_at() + 2 * prefix; }
   __host__ __device__ int64_t int4s() const { return rest_at() + rest; }
-  __host__ __device__ int64_t prefix_rows(int64_t kv_heads) const { return prefix * kv_heads * kEntryRows; }
   __host__ __device__ int64_t rows(int64_t kv_heads, int64_t group) const {
-    return prefix_rows(kv_heads) + rest * kv_heads * group;
+    return kv_heads * (prefix_rows + rest * group);
   }
 };
 __host__ __device__ constexpr int64_t slots_per_head(int64_t kv_heads) {
   return kSlots / kv_heads > 0 ? kSlots / kv_heads : 1;
 }
-// A prefix has one tile of rows or one per 128 of them, cut into at most
-// slots pieces beside one per tile; a rest one entry beside its share.
+// With tiles of S query rows a plan has at most slots + (tiles) prefix
+// entries, at most sharing + rows / S tiles, whatever S it takes.
 PlanShape plan_shape(int64_t num_seqs, int64_t num_groups, int64_t kv_heads, int64_t group,
                      int64_t rest_tokens) {
-  PlanShape p{num_seqs, 0, 0};
+  PlanShape p{num_seqs, 0, 0, 0};
   const int64_t sharing = std::min(num_groups, num_seqs / 2);
-  if (sharing > 0) p.prefix = slots_per_head(kv_heads) + sharing + num_seqs * group / kEntryRows;
+  if (sharing > 0) {
+    p.prefix = slots_per_head(kv_heads) + sharing + num_seqs * group / kMinTileRows;
+    p.prefix_rows = (slots_per_head(kv_heads) + sharing) * kTileRows + num_seqs * group;
+  }
   p.rest = slots_per_head(kv_heads) * kRestRounds;
   if (rest_tokens >= 0) p.rest = std::min(p.rest, rest_tokens / kChunk + 1);
   p.rest += num_seqs;
@@ -117,7 +137,7 @@ struct GroupOf {
     *first = s0;
     *n = s1 - s0;
     *rows = prefix[g];
-    return s0 >= 0 && s1 <= num_seqs && s1 - s0 >= 2 && *rows > 0;
+    return s0 >= 0 && s1 <= num_seqs && s1 - s0 >= 2 && *rows > 0 && *rows <= kMaxLength;
   }
   // The group of sequence i, -1 for none.
   __device__ __forceinline__ int32_t of(int32_t i) const {
@@ -146,18 +166,20 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
   const int32_t num_groups = groups.num_groups;
   // Where sequence i's own part begins: its group's prefix, when it has all of it.
   auto rest_of = [&](int32_t i, int32_t* length) {
-    *length = max(0, cu_seqlens_k[i + 1] - cu_seqlens_k[i]);
+    // (A key past the bound lies in no table; tile ends stay below 2^31.)
+    *length = min(max(0, cu_seqlens_k[i + 1] - cu_seqlens_k[i]), kMaxLength);
     const int32_t g = groups.of(i);
     int32_t first, n, rows;
     return g >= 0 && groups.shares(g, &first, &n, &rows) && *length >= rows ? rows : 0;
   };
 
+  const int32_t tile_rows = 1 << NKV_SHARED_TILE_LOG2;
   int64_t prefix_units = 0, rest_units = 0;  // 64-key tiles to walk, per kv head
   for (int32_t g = t; g < num_groups; g += kPlanThreads) {
     int32_t first, n, rows;
     if (groups.shares(g, &first, &n, &rows)) {
       const int64_t q_rows = static_cast<int64_t>(n) * group;
-      const int64_t tiles = (q_rows + kEntryRows - 1) / kEntryRows;
+      const int64_t tiles = (q_rows + tile_rows - 1) / tile_rows;
       prefix_units += tiles * ((static_cast<int64_t>(rows) + kTileKeys - 1) / kTileKeys);
     }
   }
@@ -175,7 +197,8 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
   const int64_t prefix_tiles = max(static_cast<int64_t>(kMinPrefixTiles), share);
   const int64_t room = max(static_cast<int64_t>(1), shape.rest - num_seqs);
   const int64_t rest_tiles =
-      max(max(static_cast<int64_t>(kMinRestTiles), share), (rest_units + room - 1) / room);
+      max(max(static_cast<int64_t>(kMinRestTiles), (share + kRestRounds - 1) / kRestRounds),
+          (rest_units + room - 1) / room);
   const int32_t piece_keys = static_cast<int32_t>(min(prefix_tiles, static_cast<int64_t>(1) << 24) * kTileKeys);
   const int32_t entry_keys = static_cast<int32_t>(min(rest_tiles, static_cast<int64_t>(1) << 24) * kTileKeys);
 
@@ -185,7 +208,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
       [&](int32_t g) {
         int32_t first, n, rows;
         if (!groups.shares(g, &first, &n, &rows)) return 0;
-        const int32_t tiles = (n * group + kEntryRows - 1) / kEntryRows;
+        const int32_t tiles = (n * group + tile_rows - 1) / tile_rows;
         return tiles * ((rows - 1) / piece_keys + 1);
       },
       s_mem, s_tmp);
@@ -196,14 +219,18 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
     groups.shares(g, &first, &n, &rows);
     const int32_t pieces = (rows - 1) / piece_keys + 1;
     const int32_t tile = (e - s_mem[g]) / pieces, piece = (e - s_mem[g]) % pieces;
-    const int32_t log2 = tile_log2(static_cast<int64_t>(n) * group);
+    const int32_t tile_q = min(tile_rows, n * group - tile * tile_rows);
     // Pieces of equal length, in whole tiles.
     const int32_t key_tiles = (rows - 1) / kTileKeys + 1;
     const int32_t k0 = static_cast<int32_t>(static_cast<int64_t>(key_tiles) * piece / pieces) * kTileKeys;
     const int32_t k1 = min(rows, static_cast<int32_t>(static_cast<int64_t>(key_tiles) * (piece + 1) / pieces) * kTileKeys);
     plan[shape.prefix_at() + 2 * e] =
-        make_int4(first, tile * kEntryRows, min(kEntryRows, n * group - tile * kEntryRows), log2);
-    plan[shape.prefix_at() + 2 * e + 1] = make_int4(k0, k1, 0, 0);
+        make_int4(first, tile * tile_rows, tile_q, tile_log2(tile_q));
+    plan[shape.prefix_at() + 2 * e + 1] = make_int4(k0, k1, tile_rows, n * group <= tile_rows ? 1 : 0);
+  }
+  for (int32_t e = prefix_entries + t; e < shape.prefix; e += kPlanThreads) {
+    plan[shape.prefix_at() + 2 * e] = make_int4(0, 0, 0, 0);
+    plan[shape.prefix_at() + 2 * e + 1] = make_int4(0, 0, 0, 0);
   }
   for (int32_t i = t; i < num_seqs; i += kPlanThreads) {
     const int32_t g = groups.of(i);
@@ -211,8 +238,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
     int4 record = make_int4(0, 0, 0, 0);
     if (rest_of(i, &length) > 0) {
       groups.shares(g, &first, &n, &rows);
-      record = make_int4(s_mem[g], (rows - 1) / piece_keys + 1, i - first,
-                         tile_log2(static_cast<int64_t>(n) * group));
+      record = make_int4(s_mem[g], (rows - 1) / piece_keys + 1, i - first, tile_rows);
     }
     plan[kPlanSeqs + 2 * i + 1] = record;
   }
@@ -240,6 +266,9 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
     plan[shape.rest_at() + e] =
         make_int4(i, max(start, row0), length - row0 > entry_keys ? row0 + entry_keys : length, 0);
   }
+  for (int32_t e = rest_entries + t; e < shape.rest; e += kPlanThreads) {
+    plan[shape.rest_at() + e] = make_int4(0, 0, 0, 0);
+  }
   if (t < 16) plan[2 + t] = make_int4(0, 0, 0, 0);
   if (t == 0) {
     plan[0] = make_int4(prefix_entries, rest_entries, num_seqs, num_groups);
@@ -255,12 +284,22 @@ __device__ __forceinline__ void wait_vmcnt() {
 }
 __device__ __forceinline__ void wait_lgkmcnt0() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 
+// A wave-uniform address, in scalar registers.
+__device__ __forceinline__ const uint8_t* scalar_pointer(const uint8_t* p) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a));
+  const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
+  return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(high) << 32 | low);
+}
+
+// A ring of three K tiles and two V tiles: 80 KiB, two workgroups per CU.
+// The key waves' partial sums take its place at the end, 16 KiB each, their
+// maxima and weight sums behind them.
 struct TileShared {
-  u32x4 k[2][kTileKeys * 16];
+  u32x4 k[3][kTileKeys * 16];
   u32x4 v[2][kTileKeys * 16];
-  float m[4][32];
-  float l[4][32];
 };
+static_assert(sizeof(TileShared) == 80 * 1024, "two workgroups per CU");
 
 // The cache as one item sees it: a kv head of the rows of one block table.
 struct KeySource {
@@ -272,6 +311,7 @@ struct KeySource {
   uint32_t row_bytes;
   int32_t block_size, block_shift, num_blocks;
   int32_t begin, end;  // context rows; tiles start at begin rounded down to a chunk
+  bool stream;         // no other item reads these rows: the copies pass the caches by
 };
 
 // The item's query rows [row0, row0 + rows): row r is head r % group of the
@@ -321,31 +361,38 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
     }
   }
 
-  // The block id of context row t, -1 outside the item, table or cache.
-  auto block_of = [&](int32_t t) -> int32_t {
-    const int32_t logical = src.block_shift >= 0 ? t >> src.block_shift : t / src.block_size;
+  // Blocks [window, window + 64) of the table, one id per lane, -1 outside the
+  // cache or the table: a chunk's id is a lane read, with no memory access in
+  // the loop but where a piece outgrows the window (blocks of 16 keys: every
+  // 16 tiles).
+  auto block_at = [&](int32_t t) -> int32_t {
+    return src.block_shift >= 0 ? t >> src.block_shift : t / src.block_size;
+  };
+  auto offset_at = [&](int32_t t, int32_t block) -> int32_t { return t - block * src.block_size; };
+  auto valid_id = [&](int32_t logical) -> int32_t {
     if (logical >= src.table_stride) return -1;
     const int32_t id = src.table[logical];
     return id >= 0 && id < src.num_blocks ? id : -1;
   };
-  auto offset_in_block = [&](int32_t t) -> int32_t {
-    return src.block_shift >= 0 ? t & (src.block_size - 1) : t % src.block_size;
+  const int32_t last_block = block_at(src.end - 1);
+  int32_t window = 0, ids = -1;
+  bool window_ok = false;  // every block of the item in the window is there
+  auto load_window = [&](int32_t first) {
+    window = first;
+    const int32_t logical = first + lane;
+    ids = logical <= last_block ? valid_id(logical) : -1;
+    window_ok = !__any(logical <= last_block && ids < 0);
   };
-  // Which of the 16 keys from t on are there (bit = key).
+  // Which of the 16 keys from t on are there (bit = key); the slow way, for
+  // the tiles at an item's ends and those with blocks missing.
   auto keys_there = [&](int32_t t) -> uint32_t {
-    if constexpr (kChunked) {
-      if (t >= src.end || block_of(t) < 0) return 0u;
-      const int32_t low = max(0, src.begin - t), high = min(kChunk, src.end - t);
-      return ((1u << high) - 1u) & ~((1u << low) - 1u);
-    } else {
-      const bool ok = t + c16 >= src.begin && t + c16 < src.end && block_of(t + c16) >= 0;
-      return static_cast<uint32_t>(__ballot(ok)) & 0xFFFFu;  // lanes 0-15
-    }
+    const bool ok = t + c16 >= src.begin && t + c16 < src.end && valid_id(block_at(t + c16)) >= 0;
+    return static_cast<uint32_t>(__ballot(ok)) & 0xFFFFu;  // lanes 0-15
   };
 
+  // Lane l copies 16 bytes of key 4 i + l / 16 to position l % 16 of its row.
   const uint32_t lds_k = lds_address(&sh.k[0][0]) + chunk * 4096u;
   const uint32_t lds_v = lds_address(&sh.v[0][0]) + chunk * 4096u;
-  // Lane l copies 16 bytes of key 4 i + l / 16 to position l % 16 of its row.
   uint32_t off_k[4], off_v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -353,49 +400,55 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
     off_k[i] = key * src.row_bytes + 16u * static_cast<uint32_t>(c16 ^ key);
     off_v[i] = key * src.row_bytes + 16u * static_cast<uint32_t>(c16 ^ ((key & 7) << 1));
   }
-  uint32_t there_next[NKB];
-  // Eight copies into buffer `slot`: this wavefront's chunk of the tile at t.
-  auto issue = [&](int slot, int32_t tile_t) {
-    const int32_t t = tile_t + chunk * kChunk;
-    const uint32_t dk = lds_k + slot * (kTileKeys * 256u), dv = lds_v + slot * (kTileKeys * 256u);
+  // Four copies of this wavefront's chunk of the tile at tile_t, of K or V.
+  // `row` is the chunk's cache row, -1 for a chunk that is not whole.
+  auto copy_chunk = [&](const uint8_t* head, const uint32_t* off, bool value, uint32_t dst, int32_t tile_t,
+                        int32_t row) {
+    if (row >= 0) {
+      const uint8_t* const base =
+          scalar_pointer(head + static_cast<uint64_t>(static_cast<uint32_t>(row)) * src.row_bytes);
+      if (src.stream) {
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) there_next[kb] = keys_there(tile_t + (kw * NKB + kb) * kChunk);
-    uint32_t there = there_next[0];
+        for (int i = 0; i < 4; ++i) lds_copy16<true>(base, off[i], dst + i * 1024u);
+      } else {
 #pragma unroll
-    for (int kb = 1; kb < NKB; ++kb) there = rw == kb ? there_next[kb] : there;
-    if (kChunked && there == 0xFFFFu) {
-      const int64_t row = static_cast<int64_t>(block_of(t)) * src.block_size + offset_in_block(t);
-      const uint8_t* const kr = src.k_head + row * src.row_bytes;
-      const uint8_t* const vr = src.v_head + row * src.row_bytes;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) lds_copy16<true>(kr, off_k[i], dk + i * 1024u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) lds_copy16<true>(vr, off_v[i], dv + i * 1024u);
+        for (int i = 0; i < 4; ++i) lds_copy16<false>(base, off[i], dst + i * 1024u);
+      }
     } else {
-      int64_t base[4];
+      // Keys that are not there copy zeros.
+      const int32_t t = tile_t + chunk * kChunk;
+      const uint8_t* from[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = 4 * i + g4;
-        const bool ok = (there >> key) & 1u;
-        const int32_t tk = ok ? t + key : 0;
-        const int32_t id = ok ? block_of(tk) : 0;
-        base[i] = ok ? (static_cast<int64_t>(id) * src.block_size + offset_in_block(tk)) *
-                           static_cast<int64_t>(src.row_bytes)
-                     : -1;
+        const int32_t tk = t + 4 * i + g4;
+        const bool in = tk >= src.begin && tk < src.end;
+        const int32_t block = in ? block_at(tk) : 0;
+        const int32_t id = in ? valid_id(block) : -1;
+        const uint8_t* const at = head + (static_cast<int64_t>(id) * src.block_size + offset_at(tk, block)) *
+                                             static_cast<int64_t>(src.row_bytes);
+        from[i] = id >= 0 ? at : src.zeros;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = 4 * i + g4;
-        const uint8_t* kr = base[i] >= 0 ? src.k_head + base[i] : src.zeros;
-        lds_copy16<true>(kr + 16 * (c16 ^ key), dk + i * 1024u);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 4 * i + g4;
-        const uint8_t* vr = base[i] >= 0 ? src.v_head + base[i] : src.zeros;
-        lds_copy16<true>(vr + 16 * (c16 ^ ((key & 7) << 1)), dv + i * 1024u);
+        lds_copy16<false>(from[i] + 16 * (c16 ^ (value ? (key & 7) << 1 : key)), dst + i * 1024u);
       }
     }
+  };
+  // The cache row of this wavefront's chunk of the tile at tile_t; plain: all
+  // 64 keys of the tile are there.
+  auto find_chunk = [&](int32_t tile_t, bool* plain) -> int32_t {
+    *plain = false;
+    if constexpr (!kChunked) return -1;
+    const int32_t t = tile_t + chunk * kChunk;
+    if (t >= src.end) return -1;
+    const int32_t tile_last = min(block_at(tile_t + kTileKeys - 1), last_block);
+    if (tile_last - window >= kWave) load_window(block_at(tile_t));
+    *plain = window_ok && tile_t >= src.begin && tile_t + kTileKeys <= src.end;
+    if (t < src.begin || t + kChunk > src.end) return -1;
+    const int32_t block = block_at(t);
+    const int32_t id = __builtin_amdgcn_readlane(ids, block - window);
+    return __builtin_amdgcn_readfirstlane(id >= 0 ? id * src.block_size + offset_at(t, block) : -1);
   };
 
   float row_max[NMB];
@@ -412,29 +465,13 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
 
   const int32_t first_key = src.begin & ~(kChunk - 1);
   const int32_t num_tiles = (src.end - first_key + kTileKeys - 1) / kTileKeys;
-  __builtin_amdgcn_s_waitcnt(0);  // q has landed: only the copies are in flight below
-  issue(0, first_key);
-  for (int32_t tile = 0; tile < num_tiles; ++tile) {
-    uint32_t there[NKB];
-#pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) there[kb] = there_next[kb];
-    if constexpr (RW == 1) {
-      if (tile + 1 < num_tiles) {
-        wait_lgkmcnt0();  // the other buffer has been read
-        issue((tile + 1) & 1, first_key + (tile + 1) * kTileKeys);
-        wait_vmcnt<8>();
-      } else {
-        wait_vmcnt<0>();
-      }
-    } else {
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();  // everyone's copies have landed, the other buffer has been read
-      if (tile + 1 < num_tiles) issue((tile + 1) & 1, first_key + (tile + 1) * kTileKeys);
-    }
-    const u32x4* const k_tile = sh.k[tile & 1];
-    const u32x4* const v_tile = sh.v[tile & 1];
-
-    f32x4 st[NKB][NMB];
+  auto tile_key = [&](int32_t tile) { return first_key + tile * kTileKeys; };
+  if constexpr (kChunked) load_window(block_at(first_key));
+  __builtin_amdgcn_s_waitcnt(0);  // q and ids have landed: only the copies are in flight below
+  // S^T of the tile in K slot `slot`: block (kb, mb) holds keys 16 kb + 4 g4 + i
+  // (of the wavefront's keys) of row 16 mb + c16.
+  auto scores = [&](int slot, f32x4 (&st)[NKB][NMB]) {
+    const u32x4* const k_tile = sh.k[slot];
 #pragma unroll
     for (int kb = 0; kb < NKB; ++kb) {
 #pragma unroll
@@ -446,18 +483,21 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
         for (int mb = 0; mb < NMB; ++mb) st[kb][mb] = E::mfma(a, qb[mb][dc], st[kb][mb]);
       }
     }
-    uint32_t all = 0xFFFFu;
+  };
+  // Scores to weights: -inf for the keys that are not there, the row's
+  // reference max, which moves only past kRescaleLog2, and exp2.
+  auto weights = [&](int32_t tile, bool plain, f32x4 (&st)[NKB][NMB]) {
+    if (!plain) {
 #pragma unroll
-    for (int kb = 0; kb < NKB; ++kb) all &= there[kb];
-    if (all != 0xFFFFu) {
-#pragma unroll
-      for (int kb = 0; kb < NKB; ++kb)
+      for (int kb = 0; kb < NKB; ++kb) {
+        const uint32_t there = keys_there(tile_key(tile) + (kw * NKB + kb) * kChunk);
 #pragma unroll
         for (int mb = 0; mb < NMB; ++mb)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            st[kb][mb][i] = (there[kb] >> (4 * g4 + i)) & 1u ? st[kb][mb][i] : -INFINITY;
+            st[kb][mb][i] = (there >> (4 * g4 + i)) & 1u ? st[kb][mb][i] : -INFINITY;
           }
+      }
     }
     float ref[NMB];
 #pragma unroll
@@ -478,16 +518,68 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
       }
       ref[mb] = row_max[mb] == -INFINITY ? INFINITY : row_max[mb];  // nothing yet: weights 0
     }
-    if constexpr (NKB == 1) {
-      const X4 ones = {one, one, one, one};
+#pragma unroll
+    for (int mb = 0; mb < NMB; ++mb)
+#pragma unroll
+      for (int kb = 0; kb < NKB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          st[kb][mb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kb][mb][i], scale_log2, -ref[mb]));
+        }
+  };
+
+  // Tile t's K is copied ahead of its V; within a step V goes first, so that a
+  // step waits for what it reads while the K behind it is still in flight.
+  bool plain, plain1 = false, plain2 = false, plain3 = false;  // of tiles t, t + 1, ...
+  int32_t row1 = -1, row2 = -1, row3 = -1;  // the chunk's cache row in tiles t + 1, ...
+  auto copy_k = [&](int32_t tile, int slot, int32_t row) {
+    copy_chunk(src.k_head, off_k, false, lds_k + slot * kTileBytes, tile_key(tile), row);
+  };
+  auto copy_v = [&](int32_t tile, int32_t row) {
+    copy_chunk(src.v_head, off_v, true, lds_v + (tile & 1) * kTileBytes, tile_key(tile), row);
+  };
+  {
+    const int32_t row0 = find_chunk(first_key, &plain);
+    copy_k(0, 0, row0);
+    copy_v(0, row0);
+    if (num_tiles > 1) {
+      row1 = find_chunk(tile_key(1), &plain1);
+      copy_k(1, 1, row1);
+    }
+  }
+  f32x4 st[NKB][NMB];
+  if constexpr (RW == 1) {
+    // Every wavefront reads what it copied itself: counted waits, no barrier.
+    const X4 ones = {one, one, one, one};
+    int slot = 0;  // tile % 3
+    for (int32_t tile = 0; tile < num_tiles; ++tile) {
+      const int32_t left = num_tiles - 1 - tile;  // tiles behind this one
+      if (left > 0) {
+        wait_vmcnt<8>();  // K(tile): V(tile) and K(tile + 1) may be in flight
+      } else {
+        wait_vmcnt<4>();
+      }
+      wait_lgkmcnt0();  // the slots filled next have been read
+      if (left > 0) copy_v(tile + 1, row1);
+      if (left > 1) {
+        row2 = find_chunk(tile_key(tile + 2), &plain2);
+        copy_k(tile + 2, slot == 0 ? 2 : slot - 1, row2);  // (tile + 2) % 3
+      }
+      scores(slot, st);
+      weights(tile, plain, st);
+      if (left > 1) {  // V(tile): what was issued behind it may be in flight
+        wait_vmcnt<12>();
+      } else if (left == 1) {
+        wait_vmcnt<8>();
+      } else {
+        wait_vmcnt<0>();
+      }
       X4 pb[NMB];
 #pragma unroll
       for (int mb = 0; mb < NMB; ++mb)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          pb[mb][i] = static_cast<T>(
-              __builtin_amdgcn_exp2f(__builtin_fmaf(st[0][mb][i], scale_log2, -ref[mb])));
-        }
+        for (int i = 0; i < 4; ++i) pb[mb][i] = static_cast<T>(st[0][mb][i]);
+      const u32x4* const v_tile = sh.v[tile & 1];
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
         const X4 a = __builtin_bit_cast(X4, v_tr_read(v_tile, 16 * kw + tr_key, 16 * db + tr_dim));
@@ -496,23 +588,65 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
       }
 #pragma unroll
       for (int mb = 0; mb < NMB; ++mb) acc[8][mb] = E::mfma16(ones, pb[mb], acc[8][mb]);
+      plain = plain1;
+      plain1 = plain2;
+      row1 = row2;
+      slot = slot == 2 ? 0 : slot + 1;
+    }
+  } else {
+    // A step takes tile t's weights, then, in one run of matrix instructions,
+    // the scores of tile t + 1 and tile t's product with V: while one
+    // wavefront of a SIMD is in that run, the other takes its weights.
+    const X8 ones = {one, one, one, one, one, one, one, one};
+    if (num_tiles > 2) {
+      row2 = find_chunk(tile_key(2), &plain2);
+      copy_k(2, 2, row2);
+      wait_vmcnt<12>();  // K(0)
     } else {
-      const X8 ones = {one, one, one, one, one, one, one, one};
+      wait_vmcnt<0>();
+    }
+    __syncthreads();
+    scores(0, st);
+    int slot = 0;  // tile % 3
+    for (int32_t tile = 0; tile < num_tiles; ++tile) {
+      const int32_t left = num_tiles - 1 - tile;
+      const int next = slot == 2 ? 0 : slot + 1;
+      if (left > 1) {
+        wait_vmcnt<4>();  // V(tile) and K(tile + 1): K(tile + 2) may be in flight
+      } else {
+        wait_vmcnt<0>();
+      }
+      wait_lgkmcnt0();
+      __syncthreads();  // everyone's copies have landed, the slots filled next have been read
+      if (left > 0) copy_v(tile + 1, row1);
+      if (left > 2) {
+        row3 = find_chunk(tile_key(tile + 3), &plain3);
+        copy_k(tile + 3, slot, row3);
+      }
+      weights(tile, plain, st);
       X8 pb[NKB / 2][NMB];
 #pragma unroll
       for (int mb = 0; mb < NMB; ++mb)
 #pragma unroll
-        for (int c = 0; c < NKB / 2; ++c) {
-          X8 w;
+        for (int c = 0; c < NKB / 2; ++c)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            w[i] = static_cast<T>(
-                __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * c][mb][i], scale_log2, -ref[mb])));
-            w[4 + i] = static_cast<T>(
-                __builtin_amdgcn_exp2f(__builtin_fmaf(st[2 * c + 1][mb][i], scale_log2, -ref[mb])));
+            pb[c][mb][i] = static_cast<T>(st[2 * c][mb][i]);
+            pb[c][mb][4 + i] = static_cast<T>(st[2 * c + 1][mb][i]);
           }
-          pb[c][mb] = w;
-        }
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+      __builtin_amdgcn_sched_barrier(0);
+      scores(next, st);  // (behind the last tile: of an older one, dropped)
+      // Four K operand reads ahead, then each read's products with the next read.
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < 4 * NKB; ++i) {
+        if (i < 4 * NKB - 4) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, NMB, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const u32x4* const v_tile = sh.v[tile & 1];
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
 #pragma unroll
@@ -529,6 +663,15 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
       for (int c = 0; c < NKB / 2; ++c)
 #pragma unroll
         for (int mb = 0; mb < NMB; ++mb) acc[8][mb] = E::mfma(ones, pb[c][mb], acc[8][mb]);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      plain = plain1;
+      plain1 = plain2;
+      plain2 = plain3;
+      row1 = row2;
+      row2 = row3;
+      slot = next;
     }
   }
 
@@ -548,6 +691,7 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
     __syncthreads();  // every wavefront has read its last tile
     u32x4* const buffers = reinterpret_cast<u32x4*>(&sh);  // k and v: 64 KiB in a row
     u32x4* const buffer = buffers + wave * 1024;
+    f32x2* const s_ml = reinterpret_cast<f32x2*>(buffers + 4 * 1024);  // [wavefront][row]
 #pragma unroll
     for (int mb = 0; mb < NMB; ++mb) {
       const int r = mb * 16 + c16;
@@ -555,10 +699,7 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
       for (int db = 0; db < 8; ++db) {
         buffer[r * 32 + ((4 * db + g4) ^ c16)] = __builtin_bit_cast(u32x4, acc[db][mb]);
       }
-      if (g4 == 0) {
-        sh.m[wave][r] = row_max[mb];
-        sh.l[wave][r] = acc[8][mb][0];
-      }
+      if (g4 == 0) s_ml[wave * 32 + r] = f32x2{row_max[mb], acc[8][mb][0]};
     }
     __syncthreads();
     const int total_rows = min(rows.rows, RW * NMB * 16);
@@ -567,13 +708,13 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
       const int from = row / 32, r = row & 31;  // row wave and its row
       float top = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < KW; ++k) top = fmaxf(top, sh.m[k * RW + from][r]);
+      for (int k = 0; k < KW; ++k) top = fmaxf(top, s_ml[(k * RW + from) * 32 + r].x);
       f32x4 sum = {0.f, 0.f, 0.f, 0.f};
       float l = 0.f;
 #pragma unroll
       for (int k = 0; k < KW; ++k) {
         const int w = k * RW + from;
-        const float mw = sh.m[w][r], lw = sh.l[w][r];
+        const float mw = s_ml[w * 32 + r].x, lw = s_ml[w * 32 + r].y;
         // A wavefront without keys has (-inf, 0); -inf with another sum is
         // NaN scores, which go on.
         const float f = mw == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(mw - top);
@@ -615,11 +756,8 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   __shared__ TileShared sh;
   const const_i32* const plan = (const const_i32*)a.plan;
   if (!plan_fits(plan, a.num_seqs, a.num_groups, a.num_kv_heads, a.group)) return;
-  const int32_t prefix_entries = min(static_cast<int64_t>(plan[0]), a.shape.prefix);
-  const int32_t rest_entries = min(static_cast<int64_t>(plan[1]), a.shape.rest);
   const int32_t entry = static_cast<int32_t>(blockIdx.x / static_cast<uint32_t>(a.num_kv_heads));
   const int32_t turn = static_cast<int32_t>(blockIdx.x) - entry * a.num_kv_heads;
-  if (entry >= prefix_entries + rest_entries) return;
   // The kv head rotates with the entry, so that no XCD (workgroup id % 8)
   // stays on one byte offset of the rows.
   const int32_t period = 8 / min(8, a.num_kv_heads & -a.num_kv_heads);
@@ -637,7 +775,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   rows.q = a.q + static_cast<int64_t>(kh) * a.group * kDim;
   rows.seq_stride = a.q_seq_stride;
   rows.group = a.group;
-  if (entry < prefix_entries) {
+  if (entry < a.shape.prefix) {
     const const_i32* const e = plan + 4 * (a.shape.prefix_at() + 2 * entry);
     const int32_t log2 = e[3];
     rows.first = e[0];
@@ -645,17 +783,19 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     rows.rows = e[2];
     src.begin = e[4];
     src.end = e[5];
+    src.stream = e[7] != 0;
     // Uniform exits for entries that name rows outside the batch.
-    if (rows.first < 0 || rows.row0 < 0 || rows.rows <= 0 || rows.rows > kEntryRows || src.begin < 0 ||
-        src.end <= src.begin ||
+    const int32_t tile_rows = e[6];
+    const int64_t row = static_cast<int64_t>(entry) * tile_rows;
+    if (rows.first < 0 || rows.row0 < 0 || rows.rows <= 0 || rows.rows > (1 << log2) || src.begin < 0 ||
+        src.end <= src.begin || rows.rows > tile_rows || row + rows.rows > a.shape.prefix_rows ||
         rows.first + (static_cast<int64_t>(rows.row0) + rows.rows - 1) / a.group >= a.num_seqs) {
       return;
     }
     src.table = (const const_i32*)(a.tables + static_cast<int64_t>(rows.first) * a.table_stride);
-    const int64_t row = (static_cast<int64_t>(entry) * a.num_kv_heads + kh) * kEntryRows;
-    float* const acc = a.part_acc + row * kDim;
-    f32x2* const ml = a.part_ml + row;
-    if (log2 == 7) {
+    float* const acc = a.part_acc + (kh * a.shape.prefix_rows + row) * kDim;
+    f32x2* const ml = a.part_ml + kh * a.shape.prefix_rows + row;
+    if (log2 >= 7) {
       attend<4, 2, kChunked, kHalf>(sh, src, rows, a.scale_log2, acc, ml);
     } else if (log2 == 6) {
       attend<2, 2, kChunked, kHalf>(sh, src, rows, a.scale_log2, acc, ml);
@@ -666,16 +806,17 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     }
     return;
   }
-  const int32_t s = entry - prefix_entries;
+  const int32_t s = entry - static_cast<int32_t>(a.shape.prefix);
   const const_i32* const e = plan + 4 * (a.shape.rest_at() + s);
   rows.first = e[0];
   rows.row0 = 0;
   rows.rows = a.group;
   src.begin = e[1];
   src.end = e[2];
+  src.stream = true;
   if (rows.first < 0 || rows.first >= a.num_seqs || src.begin < 0 || src.end <= src.begin) return;
   src.table = (const const_i32*)(a.tables + static_cast<int64_t>(rows.first) * a.table_stride);
-  const int64_t row = a.shape.prefix_rows(a.num_kv_heads) +
+  const int64_t row = a.num_kv_heads * a.shape.prefix_rows +
                       (static_cast<int64_t>(s) * a.num_kv_heads + kh) * a.group;
   attend<1, 1, kChunked, kHalf>(sh, src, rows, a.scale_log2, a.part_acc + row * kDim, a.part_ml + row);
 }
@@ -709,15 +850,16 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a, uint16_
   const int32_t rest_first = record[2], rest_count = record[3];
   const int32_t pieces = record[5];
   const int32_t row = record[6] * a.group + head;
-  const int32_t tile = row / kEntryRows;
-  const int64_t prefix_first = record[4] + static_cast<int64_t>(tile) * pieces;
-  const int64_t rest_row = a.shape.prefix_rows(a.num_kv_heads);
+  const int32_t tile_rows = max(1, record[7]);
+  const int32_t tile = row / tile_rows;
+  // The row's first partial; its pieces lie tile_rows apart.
+  const int64_t prefix_row = kh * a.shape.prefix_rows +
+                             (record[4] + static_cast<int64_t>(tile) * pieces) * tile_rows + row % tile_rows;
+  const int64_t prefix_most = a.num_kv_heads * a.shape.prefix_rows - 1;
+  const int64_t rest_row = a.num_kv_heads * a.shape.prefix_rows;
   const int32_t parts = pieces + rest_count;
   auto row_of = [&](int32_t p) -> int64_t {
-    if (p < pieces) {
-      const int64_t e = min(prefix_first + p, a.shape.prefix - 1);
-      return (e * a.num_kv_heads + kh) * kEntryRows + row % kEntryRows;
-    }
+    if (p < pieces) return min(prefix_row + static_cast<int64_t>(p) * tile_rows, prefix_most);
     const int64_t e = min(static_cast<int64_t>(rest_first) + p - pieces, a.shape.rest - 1);
     return rest_row + (e * a.num_kv_heads + kh) * a.group + head;
   };
