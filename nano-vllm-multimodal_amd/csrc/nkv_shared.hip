@@ -362,17 +362,11 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
   }
 
   // Blocks [window, window + 64) of the table, one id per lane, -1 outside the
-  // cache or the table: a chunk's id is a lane read, with no memory access in
-  // the loop but where a piece outgrows the window (blocks of 16 keys: every
-  // 16 tiles).
+  // cache or the table: a tile's keys find their rows by lane reads, with no
+  // memory access in the loop but where an item outgrows the window (blocks
+  // of 16 keys: every 16 tiles).
   auto block_at = [&](int32_t t) -> int32_t {
     return src.block_shift >= 0 ? t >> src.block_shift : t / src.block_size;
-  };
-  auto offset_at = [&](int32_t t, int32_t block) -> int32_t { return t - block * src.block_size; };
-  auto valid_id = [&](int32_t logical) -> int32_t {
-    if (logical >= src.table_stride) return -1;
-    const int32_t id = src.table[logical];
-    return id >= 0 && id < src.num_blocks ? id : -1;
   };
   const int32_t last_block = block_at(src.end - 1);
   int32_t window = 0, ids = -1;
@@ -380,14 +374,49 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
   auto load_window = [&](int32_t first) {
     window = first;
     const int32_t logical = first + lane;
-    ids = logical <= last_block ? valid_id(logical) : -1;
+    ids = -1;
+    if (logical <= last_block && logical < src.table_stride) {
+      ids = src.table[logical];
+      if (ids >= src.num_blocks) ids = -1;
+    }
     window_ok = !__any(logical <= last_block && ids < 0);
   };
-  // Which of the 16 keys from t on are there (bit = key); the slow way, for
-  // the tiles at an item's ends and those with blocks missing.
-  auto keys_there = [&](int32_t t) -> uint32_t {
-    const bool ok = t + c16 >= src.begin && t + c16 < src.end && valid_id(block_at(t + c16)) >= 0;
-    return static_cast<uint32_t>(__ballot(ok)) & 0xFFFFu;  // lanes 0-15
+  // What is known of a tile from the copies of its K to its products: its
+  // keys that are there (bit = key) and where this wavefront's chunk lies (a
+  // cache row for its first key; without whole chunks a row for each of the
+  // lane's four keys).
+  struct Tile {
+    uint64_t there;
+    int32_t row[kChunked ? 1 : 4];
+  };
+  auto find = [&](int32_t tile_t) -> Tile {
+    Tile tile;
+    const int32_t tile_last = min(block_at(tile_t + kTileKeys - 1), last_block);
+    if (tile_last - window >= kWave) load_window(block_at(tile_t));
+    const bool inside = tile_t >= src.begin && tile_t + kTileKeys <= src.end;
+    if constexpr (kChunked) {
+      const int32_t t = tile_t + chunk * kChunk;
+      const int32_t block = block_at(t);
+      const int32_t id = __builtin_amdgcn_readlane(ids, (block - window) & (kWave - 1));
+      tile.row[0] = __builtin_amdgcn_readfirstlane(
+          t < src.end && id >= 0 ? id * src.block_size + (t - block * src.block_size) : 0);
+      tile.there = ~uint64_t{0};
+      if (!inside || !window_ok) {
+        const int32_t key = tile_t + lane;
+        const int32_t mine = __shfl(ids, (block_at(key) - window) & (kWave - 1), kWave);
+        tile.there = __ballot(key >= src.begin && key < src.end && mine >= 0);
+      }
+    } else {
+      const int32_t key = tile_t + lane;
+      const int32_t block = block_at(key);
+      const int32_t mine = __shfl(ids, (block - window) & (kWave - 1), kWave);
+      const bool ok = key >= src.begin && key < src.end && mine >= 0;
+      tile.there = __ballot(ok);
+      const int32_t row = ok ? mine * src.block_size + (key - block * src.block_size) : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tile.row[i] = __shfl(row, chunk * kChunk + 4 * i + g4, kWave);
+    }
+    return tile;
   };
 
   // Lane l copies 16 bytes of key 4 i + l / 16 to position l % 16 of its row.
@@ -400,13 +429,13 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
     off_k[i] = key * src.row_bytes + 16u * static_cast<uint32_t>(c16 ^ key);
     off_v[i] = key * src.row_bytes + 16u * static_cast<uint32_t>(c16 ^ ((key & 7) << 1));
   }
-  // Four copies of this wavefront's chunk of the tile at tile_t, of K or V.
-  // `row` is the chunk's cache row, -1 for a chunk that is not whole.
-  auto copy_chunk = [&](const uint8_t* head, const uint32_t* off, bool value, uint32_t dst, int32_t tile_t,
-                        int32_t row) {
-    if (row >= 0) {
+  // Four copies of this wavefront's chunk of a tile, of K or V.  Keys that are
+  // not there copy zeros.
+  auto copy_chunk = [&](const uint8_t* head, const uint32_t* off, uint32_t dst, const Tile& tile) {
+    const uint32_t there = static_cast<uint32_t>(tile.there >> (chunk * kChunk)) & 0xFFFFu;
+    if (kChunked && there == 0xFFFFu) {
       const uint8_t* const base =
-          scalar_pointer(head + static_cast<uint64_t>(static_cast<uint32_t>(row)) * src.row_bytes);
+          scalar_pointer(head + static_cast<uint64_t>(static_cast<uint32_t>(tile.row[0])) * src.row_bytes);
       if (src.stream) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) lds_copy16<true>(base, off[i], dst + i * 1024u);
@@ -415,40 +444,17 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
         for (int i = 0; i < 4; ++i) lds_copy16<false>(base, off[i], dst + i * 1024u);
       }
     } else {
-      // Keys that are not there copy zeros.
-      const int32_t t = tile_t + chunk * kChunk;
-      const uint8_t* from[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int32_t tk = t + 4 * i + g4;
-        const bool in = tk >= src.begin && tk < src.end;
-        const int32_t block = in ? block_at(tk) : 0;
-        const int32_t id = in ? valid_id(block) : -1;
-        const uint8_t* const at = head + (static_cast<int64_t>(id) * src.block_size + offset_at(tk, block)) *
-                                             static_cast<int64_t>(src.row_bytes);
-        from[i] = id >= 0 ? at : src.zeros;
-      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int key = 4 * i + g4;
-        lds_copy16<false>(from[i] + 16 * (c16 ^ (value ? (key & 7) << 1 : key)), dst + i * 1024u);
+        // off[i] is the key's row from the chunk's first and the place in it.
+        const uint32_t place = off[i] - key * src.row_bytes;
+        const int32_t row = kChunked ? tile.row[0] + key : tile.row[kChunked ? 0 : i];
+        const uint8_t* const from =
+            (there >> key) & 1u ? head + static_cast<uint64_t>(static_cast<uint32_t>(row)) * src.row_bytes : src.zeros;
+        lds_copy16<false>(from + place, dst + i * 1024u);
       }
     }
-  };
-  // The cache row of this wavefront's chunk of the tile at tile_t; plain: all
-  // 64 keys of the tile are there.
-  auto find_chunk = [&](int32_t tile_t, bool* plain) -> int32_t {
-    *plain = false;
-    if constexpr (!kChunked) return -1;
-    const int32_t t = tile_t + chunk * kChunk;
-    if (t >= src.end) return -1;
-    const int32_t tile_last = min(block_at(tile_t + kTileKeys - 1), last_block);
-    if (tile_last - window >= kWave) load_window(block_at(tile_t));
-    *plain = window_ok && tile_t >= src.begin && tile_t + kTileKeys <= src.end;
-    if (t < src.begin || t + kChunk > src.end) return -1;
-    const int32_t block = block_at(t);
-    const int32_t id = __builtin_amdgcn_readlane(ids, block - window);
-    return __builtin_amdgcn_readfirstlane(id >= 0 ? id * src.block_size + offset_at(t, block) : -1);
   };
 
   float row_max[NMB];
@@ -466,7 +472,7 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
   const int32_t first_key = src.begin & ~(kChunk - 1);
   const int32_t num_tiles = (src.end - first_key + kTileKeys - 1) / kTileKeys;
   auto tile_key = [&](int32_t tile) { return first_key + tile * kTileKeys; };
-  if constexpr (kChunked) load_window(block_at(first_key));
+  load_window(block_at(first_key));
   __builtin_amdgcn_s_waitcnt(0);  // q and ids have landed: only the copies are in flight below
   // S^T of the tile in K slot `slot`: block (kb, mb) holds keys 16 kb + 4 g4 + i
   // (of the wavefront's keys) of row 16 mb + c16.
@@ -486,17 +492,15 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
   };
   // Scores to weights: -inf for the keys that are not there, the row's
   // reference max, which moves only past kRescaleLog2, and exp2.
-  auto weights = [&](int32_t tile, bool plain, f32x4 (&st)[NKB][NMB]) {
-    if (!plain) {
+  auto weights = [&](uint64_t tile_there, f32x4 (&st)[NKB][NMB]) {
+    if (tile_there != ~uint64_t{0}) {
 #pragma unroll
       for (int kb = 0; kb < NKB; ++kb) {
-        const uint32_t there = keys_there(tile_key(tile) + (kw * NKB + kb) * kChunk);
+        const uint32_t there = static_cast<uint32_t>(tile_there >> ((kw * NKB + kb) * kChunk)) >> (4 * g4);
 #pragma unroll
         for (int mb = 0; mb < NMB; ++mb)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            st[kb][mb][i] = (there >> (4 * g4 + i)) & 1u ? st[kb][mb][i] : -INFINITY;
-          }
+          for (int i = 0; i < 4; ++i) st[kb][mb][i] = (there >> i) & 1u ? st[kb][mb][i] : -INFINITY;
       }
     }
     float ref[NMB];
@@ -530,22 +534,19 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
 
   // Tile t's K is copied ahead of its V; within a step V goes first, so that a
   // step waits for what it reads while the K behind it is still in flight.
-  bool plain, plain1 = false, plain2 = false, plain3 = false;  // of tiles t, t + 1, ...
-  int32_t row1 = -1, row2 = -1, row3 = -1;  // the chunk's cache row in tiles t + 1, ...
-  auto copy_k = [&](int32_t tile, int slot, int32_t row) {
-    copy_chunk(src.k_head, off_k, false, lds_k + slot * kTileBytes, tile_key(tile), row);
+  Tile now{}, ahead1{}, ahead2{}, ahead3{};  // tiles t, t + 1, ...
+  auto copy_k = [&](int slot, const Tile& tile) {
+    copy_chunk(src.k_head, off_k, lds_k + slot * kTileBytes, tile);
   };
-  auto copy_v = [&](int32_t tile, int32_t row) {
-    copy_chunk(src.v_head, off_v, true, lds_v + (tile & 1) * kTileBytes, tile_key(tile), row);
+  auto copy_v = [&](int32_t t, const Tile& tile) {
+    copy_chunk(src.v_head, off_v, lds_v + (t & 1) * kTileBytes, tile);
   };
-  {
-    const int32_t row0 = find_chunk(first_key, &plain);
-    copy_k(0, 0, row0);
-    copy_v(0, row0);
-    if (num_tiles > 1) {
-      row1 = find_chunk(tile_key(1), &plain1);
-      copy_k(1, 1, row1);
-    }
+  now = find(first_key);
+  copy_k(0, now);
+  copy_v(0, now);
+  if (num_tiles > 1) {
+    ahead1 = find(tile_key(1));
+    copy_k(1, ahead1);
   }
   f32x4 st[NKB][NMB];
   if constexpr (RW == 1) {
@@ -560,13 +561,13 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
         wait_vmcnt<4>();
       }
       wait_lgkmcnt0();  // the slots filled next have been read
-      if (left > 0) copy_v(tile + 1, row1);
+      if (left > 0) copy_v(tile + 1, ahead1);
       if (left > 1) {
-        row2 = find_chunk(tile_key(tile + 2), &plain2);
-        copy_k(tile + 2, slot == 0 ? 2 : slot - 1, row2);  // (tile + 2) % 3
+        ahead2 = find(tile_key(tile + 2));
+        copy_k(slot == 0 ? 2 : slot - 1, ahead2);  // (tile + 2) % 3
       }
       scores(slot, st);
-      weights(tile, plain, st);
+      weights(now.there, st);
       if (left > 1) {  // V(tile): what was issued behind it may be in flight
         wait_vmcnt<12>();
       } else if (left == 1) {
@@ -588,9 +589,8 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
       }
 #pragma unroll
       for (int mb = 0; mb < NMB; ++mb) acc[8][mb] = E::mfma16(ones, pb[mb], acc[8][mb]);
-      plain = plain1;
-      plain1 = plain2;
-      row1 = row2;
+      now = ahead1;
+      ahead1 = ahead2;
       slot = slot == 2 ? 0 : slot + 1;
     }
   } else {
@@ -599,8 +599,8 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
     // wavefront of a SIMD is in that run, the other takes its weights.
     const X8 ones = {one, one, one, one, one, one, one, one};
     if (num_tiles > 2) {
-      row2 = find_chunk(tile_key(2), &plain2);
-      copy_k(2, 2, row2);
+      ahead2 = find(tile_key(2));
+      copy_k(2, ahead2);
       wait_vmcnt<12>();  // K(0)
     } else {
       wait_vmcnt<0>();
@@ -618,12 +618,12 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
       }
       wait_lgkmcnt0();
       __syncthreads();  // everyone's copies have landed, the slots filled next have been read
-      if (left > 0) copy_v(tile + 1, row1);
+      if (left > 0) copy_v(tile + 1, ahead1);
       if (left > 2) {
-        row3 = find_chunk(tile_key(tile + 3), &plain3);
-        copy_k(tile + 3, slot, row3);
+        ahead3 = find(tile_key(tile + 3));
+        copy_k(slot, ahead3);
       }
-      weights(tile, plain, st);
+      weights(now.there, st);
       X8 pb[NKB / 2][NMB];
 #pragma unroll
       for (int mb = 0; mb < NMB; ++mb)
@@ -666,11 +666,9 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
-      plain = plain1;
-      plain1 = plain2;
-      plain2 = plain3;
-      row1 = row2;
-      row2 = row3;
+      now = ahead1;
+      ahead1 = ahead2;
+      ahead2 = ahead3;
       slot = next;
     }
   }
