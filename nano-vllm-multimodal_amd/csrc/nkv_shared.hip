@@ -51,17 +51,17 @@ constexpr int kMinTileRows = 32;  // ... and at least, where a group has more
 constexpr int kPlanThreads = 1024;
 constexpr int kSlots = 512;       // workgroups resident on the chip: two per CU
 #ifndef NKV_SHARED_REST_ROUNDS
-#define NKV_SHARED_REST_ROUNDS 4  // entries of the rests: about so many rounds of workgroups
+#define NKV_SHARED_REST_ROUNDS 4  // entries of the rests: about so many rounds of wavefronts
 #endif
 #ifndef NKV_SHARED_MIN_PREFIX
 #define NKV_SHARED_MIN_PREFIX 2  // shortest piece of a prefix, in 64-key tiles
 #endif
 #ifndef NKV_SHARED_MIN_REST
-#define NKV_SHARED_MIN_REST 2  // shortest entry of a rest
+#define NKV_SHARED_MIN_REST 4  // shortest entry of a rest, in 16-key chunks
 #endif
 constexpr int kRestRounds = NKV_SHARED_REST_ROUNDS;
 constexpr int kMinPrefixTiles = NKV_SHARED_MIN_PREFIX;
-constexpr int kMinRestTiles = NKV_SHARED_MIN_REST;
+constexpr int kMinRestChunks = NKV_SHARED_MIN_REST;
 constexpr int32_t kMaxLength = 0x7FFFFF00;
 constexpr float kRescaleLog2 = 8.f;  // the reference max moves only past this
 
@@ -106,7 +106,7 @@ PlanShape plan_shape(int64_t num_seqs, int64_t num_groups, int64_t kv_heads, int
     p.prefix = slots_per_head(kv_heads) + sharing + num_seqs * group / kMinTileRows;
     p.prefix_rows = (slots_per_head(kv_heads) + sharing) * kTileRows + num_seqs * group;
   }
-  p.rest = slots_per_head(kv_heads) * kRestRounds;
+  p.rest = 4 * slots_per_head(kv_heads) * kRestRounds;
   if (rest_tokens >= 0) p.rest = std::min(p.rest, rest_tokens / kChunk + 1);
   p.rest += num_seqs;
   return p;
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
   };
 
   const int32_t tile_rows = 1 << NKV_SHARED_TILE_LOG2;
-  int64_t prefix_units = 0, rest_units = 0;  // 64-key tiles to walk, per kv head
+  int64_t prefix_units = 0, rest_units = 0;  // 64-key tiles and 16-key chunks to walk, per kv head
   for (int32_t g = t; g < num_groups; g += kPlanThreads) {
     int32_t first, n, rows;
     if (groups.shares(g, &first, &n, &rows)) {
@@ -186,21 +186,21 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
   for (int32_t i = t; i < num_seqs; i += kPlanThreads) {
     int32_t length;
     const int32_t start = rest_of(i, &length);
-    if (length > start) rest_units += (static_cast<int64_t>(length) - (start & -kChunk) + kTileKeys - 1) / kTileKeys;
+    if (length > start) rest_units += (static_cast<int64_t>(length) - (start & -kChunk) + kChunk - 1) / kChunk;
   }
   prefix_units = block_sum(prefix_units, s_sum);
   rest_units = block_sum(rest_units, s_sum);
-  // Tiles per piece: all items together one round of workgroups.  The rests'
-  // entries are bounded by the plan's room for them.
+  // Prefixes: all items together one round of workgroups.  Rests: about
+  // kRestRounds rounds of wavefronts, within the plan's room for them.
   const int64_t slots = slots_per_head(num_kv_heads);
-  const int64_t share = (prefix_units + rest_units + slots - 1) / slots;
+  const int64_t share = (prefix_units + rest_units / 4 + slots - 1) / slots;
   const int64_t prefix_tiles = max(static_cast<int64_t>(kMinPrefixTiles), share);
   const int64_t room = max(static_cast<int64_t>(1), shape.rest - num_seqs);
-  const int64_t rest_tiles =
-      max(max(static_cast<int64_t>(kMinRestTiles), (share + kRestRounds - 1) / kRestRounds),
+  const int64_t rest_chunks =
+      max(max(static_cast<int64_t>(kMinRestChunks), rest_units / (4 * slots * kRestRounds) + 1),
           (rest_units + room - 1) / room);
   const int32_t piece_keys = static_cast<int32_t>(min(prefix_tiles, static_cast<int64_t>(1) << 24) * kTileKeys);
-  const int32_t entry_keys = static_cast<int32_t>(min(rest_tiles, static_cast<int64_t>(1) << 24) * kTileKeys);
+  const int32_t entry_keys = static_cast<int32_t>(min(rest_chunks, static_cast<int64_t>(1) << 26) * kChunk);
 
   // Prefix entries: a group's tiles of query rows, each cut into pieces.
   lds_exclusive_scan<kPlanThreads>(
@@ -322,6 +322,91 @@ struct RowSource {
   int32_t first, row0, rows, group;
 };
 
+// Blocks [first, first + 64) of an item's table, one id per lane, -1 outside
+// the cache or the table: keys find their rows by lane reads, with no memory
+// access in the loop but where an item outgrows the window (blocks of 16
+// keys: every 1,024 keys).
+struct BlockWindow {
+  const KeySource& src;
+  int32_t last, first, ids;
+  bool ok;  // every block of the item in the window is there
+  __device__ __forceinline__ explicit BlockWindow(const KeySource& s) : src(s), first(0), ids(-1), ok(false) {
+    last = block_at(src.end - 1);
+  }
+  __device__ __forceinline__ int32_t block_at(int32_t t) const {
+    return src.block_shift >= 0 ? t >> src.block_shift : t / src.block_size;
+  }
+  __device__ __forceinline__ void load(int32_t block) {
+    first = block;
+    const int32_t logical = block + static_cast<int32_t>(threadIdx.x & (kWave - 1));
+    ids = -1;
+    if (logical <= last && logical < src.table_stride) {
+      ids = src.table[logical];
+      if (ids >= src.num_blocks) ids = -1;
+    }
+    ok = !__any(logical <= last && ids < 0);
+  }
+  // Makes the window hold the blocks of keys [t, t + keys).
+  __device__ __forceinline__ void cover(int32_t t, int32_t keys) {
+    if (min(block_at(t + keys - 1), last) - first >= kWave) load(block_at(t));
+  }
+  // The cache row of the lane's key, -1 if it is not there.
+  __device__ __forceinline__ int32_t row_of(int32_t key) const {
+    const int32_t block = block_at(key);
+    const int32_t id = __shfl(ids, (block - first) & (kWave - 1), kWave);
+    return key >= src.begin && key < src.end && id >= 0 ? id * src.block_size + (key - block * src.block_size) : -1;
+  }
+};
+
+// Four copies of a 16-key chunk of K or V into LDS: lane l copies 16 bytes of
+// key 4 i + l / 16 to position l % 16 of its row.  Keys that are not there
+// (their bit in `there` is 0) copy zeros.  row: the cache row of the chunk's
+// first key, or, without whole chunks, of the lane's four keys.
+template <bool kChunked>
+struct ChunkCopy {
+  const KeySource& src;
+  int c16, g4;
+  uint32_t off_k[4], off_v[4];
+  __device__ __forceinline__ ChunkCopy(const KeySource& s, int lane) : src(s), c16(lane & 15), g4(lane >> 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = 4 * i + g4;
+      off_k[i] = key * src.row_bytes + 16u * static_cast<uint32_t>(c16 ^ key);
+      off_v[i] = key * src.row_bytes + 16u * static_cast<uint32_t>(c16 ^ ((key & 7) << 1));
+    }
+  }
+  __device__ __forceinline__ void run(const uint8_t* head, const uint32_t* off, uint32_t dst, uint32_t there,
+                                      const int32_t* row) const {
+    if (kChunked && there == 0xFFFFu) {
+      const uint8_t* const base =
+          scalar_pointer(head + static_cast<uint64_t>(static_cast<uint32_t>(row[0])) * src.row_bytes);
+      if (src.stream) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds_copy16<true>(base, off[i], dst + i * 1024u);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lds_copy16<false>(base, off[i], dst + i * 1024u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 4 * i + g4;
+        const uint32_t place = off[i] - key * src.row_bytes;  // inside the key's row
+        const int32_t at = kChunked ? row[0] + key : row[kChunked ? 0 : i];
+        const uint8_t* const from =
+            (there >> key) & 1u ? head + static_cast<uint64_t>(static_cast<uint32_t>(at)) * src.row_bytes : src.zeros;
+        lds_copy16<false>(from + place, dst + i * 1024u);
+      }
+    }
+  }
+  __device__ __forceinline__ void k(uint32_t dst, uint32_t there, const int32_t* row) const {
+    run(src.k_head, off_k, dst, there, row);
+  }
+  __device__ __forceinline__ void v(uint32_t dst, uint32_t there, const int32_t* row) const {
+    run(src.v_head, off_v, dst, there, row);
+  }
+};
+
 // kChunked: blocks are whole 16-key chunks (one block id per chunk, read as a
 // scalar); otherwise every key looks up its own.
 template <int RW, int NMB, bool kChunked, bool kHalf>
@@ -361,26 +446,7 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
     }
   }
 
-  // Blocks [window, window + 64) of the table, one id per lane, -1 outside the
-  // cache or the table: a tile's keys find their rows by lane reads, with no
-  // memory access in the loop but where an item outgrows the window (blocks
-  // of 16 keys: every 16 tiles).
-  auto block_at = [&](int32_t t) -> int32_t {
-    return src.block_shift >= 0 ? t >> src.block_shift : t / src.block_size;
-  };
-  const int32_t last_block = block_at(src.end - 1);
-  int32_t window = 0, ids = -1;
-  bool window_ok = false;  // every block of the item in the window is there
-  auto load_window = [&](int32_t first) {
-    window = first;
-    const int32_t logical = first + lane;
-    ids = -1;
-    if (logical <= last_block && logical < src.table_stride) {
-      ids = src.table[logical];
-      if (ids >= src.num_blocks) ids = -1;
-    }
-    window_ok = !__any(logical <= last_block && ids < 0);
-  };
+  BlockWindow window(src);
   // What is known of a tile from the copies of its K to its products: its
   // keys that are there (bit = key) and where this wavefront's chunk lies (a
   // cache row for its first key; without whole chunks a row for each of the
@@ -391,71 +457,28 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
   };
   auto find = [&](int32_t tile_t) -> Tile {
     Tile tile;
-    const int32_t tile_last = min(block_at(tile_t + kTileKeys - 1), last_block);
-    if (tile_last - window >= kWave) load_window(block_at(tile_t));
-    const bool inside = tile_t >= src.begin && tile_t + kTileKeys <= src.end;
+    window.cover(tile_t, kTileKeys);
     if constexpr (kChunked) {
       const int32_t t = tile_t + chunk * kChunk;
-      const int32_t block = block_at(t);
-      const int32_t id = __builtin_amdgcn_readlane(ids, (block - window) & (kWave - 1));
+      const int32_t block = window.block_at(t);
+      const int32_t id = __builtin_amdgcn_readlane(window.ids, (block - window.first) & (kWave - 1));
       tile.row[0] = __builtin_amdgcn_readfirstlane(
           t < src.end && id >= 0 ? id * src.block_size + (t - block * src.block_size) : 0);
       tile.there = ~uint64_t{0};
-      if (!inside || !window_ok) {
-        const int32_t key = tile_t + lane;
-        const int32_t mine = __shfl(ids, (block_at(key) - window) & (kWave - 1), kWave);
-        tile.there = __ballot(key >= src.begin && key < src.end && mine >= 0);
+      if (tile_t < src.begin || tile_t + kTileKeys > src.end || !window.ok) {
+        tile.there = __ballot(window.row_of(tile_t + lane) >= 0);
       }
     } else {
-      const int32_t key = tile_t + lane;
-      const int32_t block = block_at(key);
-      const int32_t mine = __shfl(ids, (block - window) & (kWave - 1), kWave);
-      const bool ok = key >= src.begin && key < src.end && mine >= 0;
-      tile.there = __ballot(ok);
-      const int32_t row = ok ? mine * src.block_size + (key - block * src.block_size) : 0;
+      const int32_t row = window.row_of(tile_t + lane);
+      tile.there = __ballot(row >= 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) tile.row[i] = __shfl(row, chunk * kChunk + 4 * i + g4, kWave);
     }
     return tile;
   };
-
-  // Lane l copies 16 bytes of key 4 i + l / 16 to position l % 16 of its row.
+  const ChunkCopy<kChunked> copy(src, lane);
   const uint32_t lds_k = lds_address(&sh.k[0][0]) + chunk * 4096u;
   const uint32_t lds_v = lds_address(&sh.v[0][0]) + chunk * 4096u;
-  uint32_t off_k[4], off_v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int key = 4 * i + g4;
-    off_k[i] = key * src.row_bytes + 16u * static_cast<uint32_t>(c16 ^ key);
-    off_v[i] = key * src.row_bytes + 16u * static_cast<uint32_t>(c16 ^ ((key & 7) << 1));
-  }
-  // Four copies of this wavefront's chunk of a tile, of K or V.  Keys that are
-  // not there copy zeros.
-  auto copy_chunk = [&](const uint8_t* head, const uint32_t* off, uint32_t dst, const Tile& tile) {
-    const uint32_t there = static_cast<uint32_t>(tile.there >> (chunk * kChunk)) & 0xFFFFu;
-    if (kChunked && there == 0xFFFFu) {
-      const uint8_t* const base =
-          scalar_pointer(head + static_cast<uint64_t>(static_cast<uint32_t>(tile.row[0])) * src.row_bytes);
-      if (src.stream) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) lds_copy16<true>(base, off[i], dst + i * 1024u);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) lds_copy16<false>(base, off[i], dst + i * 1024u);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 4 * i + g4;
-        // off[i] is the key's row from the chunk's first and the place in it.
-        const uint32_t place = off[i] - key * src.row_bytes;
-        const int32_t row = kChunked ? tile.row[0] + key : tile.row[kChunked ? 0 : i];
-        const uint8_t* const from =
-            (there >> key) & 1u ? head + static_cast<uint64_t>(static_cast<uint32_t>(row)) * src.row_bytes : src.zeros;
-        lds_copy16<false>(from + place, dst + i * 1024u);
-      }
-    }
-  };
 
   float row_max[NMB];
   f32x4 acc[9][NMB];  // dims 16 db + 4 g4 + i of row c16; block 8: the weight sum (g4 == 0, i == 0)
@@ -472,7 +495,7 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
   const int32_t first_key = src.begin & ~(kChunk - 1);
   const int32_t num_tiles = (src.end - first_key + kTileKeys - 1) / kTileKeys;
   auto tile_key = [&](int32_t tile) { return first_key + tile * kTileKeys; };
-  load_window(block_at(first_key));
+  window.load(window.block_at(first_key));
   __builtin_amdgcn_s_waitcnt(0);  // q and ids have landed: only the copies are in flight below
   // S^T of the tile in K slot `slot`: block (kb, mb) holds keys 16 kb + 4 g4 + i
   // (of the wavefront's keys) of row 16 mb + c16.
@@ -536,10 +559,10 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
   // step waits for what it reads while the K behind it is still in flight.
   Tile now{}, ahead1{}, ahead2{}, ahead3{};  // tiles t, t + 1, ...
   auto copy_k = [&](int slot, const Tile& tile) {
-    copy_chunk(src.k_head, off_k, lds_k + slot * kTileBytes, tile);
+    copy.k(lds_k + slot * kTileBytes, static_cast<uint32_t>(tile.there >> (chunk * kChunk)) & 0xFFFFu, tile.row);
   };
   auto copy_v = [&](int32_t t, const Tile& tile) {
-    copy_chunk(src.v_head, off_v, lds_v + (t & 1) * kTileBytes, tile);
+    copy.v(lds_v + (t & 1) * kTileBytes, static_cast<uint32_t>(tile.there >> (chunk * kChunk)) & 0xFFFFu, tile.row);
   };
   now = find(first_key);
   copy_k(0, now);
@@ -729,6 +752,149 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
   }
 }
 
+// A sequence's rest, by one wavefront on its own: the group's query heads (at
+// most 16 rows) over [begin, end) in 16-key chunks, K two chunks ahead and V
+// one in a ring of its own (20 KiB).  A rest is short next to what starting an
+// item costs (its entry, block ids, q and first chunk, one after another,
+// 2.5 us, and its partial 1.2): four wavefronts that each walk an item overlap
+// these where one workgroup per item waited for them (2,640 items of 5.7
+// 64-key tiles took 10 us each, 4.3 of them so).
+constexpr int kSoloBytes = 20 * 1024;
+template <bool kChunked, bool kHalf>
+__device__ __forceinline__ void attend_solo(TileShared& sh, const KeySource& src, const uint16_t* q,
+                                            int32_t group, float scale_log2, float* __restrict__ part_acc,
+                                            f32x2* __restrict__ part_ml) {
+  typedef Elem<kHalf> E;
+  typedef typename E::T T;
+  typedef typename E::X8 X8;
+  typedef typename E::X4 X4;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int c16 = lane & 15;
+  const int g4 = lane >> 4;
+  X8 qb[4];
+  {
+    const uint16_t* row = q + (c16 < group ? c16 : 0) * kDim;
+#pragma unroll
+    for (int dc = 0; dc < 4; ++dc) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (c16 < group) v = *reinterpret_cast<const u32x4*>(row + 32 * dc + 8 * g4);
+      qb[dc] = __builtin_bit_cast(X8, v);
+    }
+  }
+  BlockWindow window(src);
+  const int32_t first_key = src.begin & ~(kChunk - 1);
+  const int32_t chunks = (src.end - first_key + kChunk - 1) / kChunk;
+  window.load(window.block_at(first_key));
+  struct Chunk {
+    uint32_t there;
+    int32_t row[kChunked ? 1 : 4];
+  };
+  auto find = [&](int32_t t) -> Chunk {
+    Chunk c;
+    window.cover(t, kChunk);
+    if constexpr (kChunked) {
+      const int32_t block = window.block_at(t);
+      const int32_t id = __builtin_amdgcn_readlane(window.ids, (block - window.first) & (kWave - 1));
+      const int32_t low = max(0, src.begin - t), high = min(kChunk, src.end - t);
+      c.there = id >= 0 ? ((1u << high) - 1u) & ~((1u << low) - 1u) : 0u;
+      c.row[0] = __builtin_amdgcn_readfirstlane(id >= 0 ? id * src.block_size + (t - block * src.block_size) : 0);
+    } else {
+      const int32_t key = t + c16;
+      const int32_t row = window.row_of(key);
+      c.there = static_cast<uint32_t>(__ballot(row >= 0)) & 0xFFFFu;  // lanes 0-15
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c.row[i] = __shfl(row, 4 * i + g4, kWave);
+    }
+    return c;
+  };
+  const ChunkCopy<kChunked> copy(src, lane);
+  const uint32_t lds_k = lds_address(reinterpret_cast<const u32x4*>(&sh)) + wave * kSoloBytes;
+  const uint32_t lds_v = lds_k + 3 * 4096u;
+  const u32x4* const ring = reinterpret_cast<const u32x4*>(&sh) + wave * (kSoloBytes / 16);
+
+  float row_max = -INFINITY;
+  f32x4 acc[9];
+#pragma unroll
+  for (int db = 0; db < 9; ++db) acc[db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const T one = c16 == 0 ? static_cast<T>(1.f) : static_cast<T>(0.f);
+  const X4 ones = {one, one, one, one};
+  const int tr_key = 4 * g4 + ((lane >> 2) & 3);
+  const int tr_dim = 4 * (lane & 3);
+
+  __builtin_amdgcn_s_waitcnt(0);  // q and ids have landed: only the copies are in flight below
+  Chunk now = find(first_key), ahead1{}, ahead2{};
+  copy.k(lds_k, now.there, now.row);
+  copy.v(lds_v, now.there, now.row);
+  if (chunks > 1) {
+    ahead1 = find(first_key + kChunk);
+    copy.k(lds_k + 4096u, ahead1.there, ahead1.row);
+  }
+  int slot = 0;  // chunk % 3
+  for (int32_t c = 0; c < chunks; ++c) {
+    const int32_t left = chunks - 1 - c;
+    if (left > 0) {
+      wait_vmcnt<8>();  // K(c): V(c) and K(c + 1) may be in flight
+    } else {
+      wait_vmcnt<4>();
+    }
+    wait_lgkmcnt0();  // the slots filled next have been read
+    if (left > 0) copy.v(lds_v + ((c + 1) & 1) * 4096u, ahead1.there, ahead1.row);
+    if (left > 1) {
+      ahead2 = find(first_key + (c + 2) * kChunk);
+      copy.k(lds_k + (slot == 0 ? 2 : slot - 1) * 4096u, ahead2.there, ahead2.row);  // (c + 2) % 3
+    }
+    const u32x4* const k_tile = ring + slot * 256;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dc = 0; dc < 4; ++dc) {
+      s = E::mfma(__builtin_bit_cast(X8, k_tile[k_index(c16, 4 * dc + g4)]), qb[dc], s);
+    }
+    if (now.there != 0xFFFFu) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] = (now.there >> (4 * g4 + i)) & 1u ? s[i] : -INFINITY;
+    }
+    float local = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    local = row4_max(local) * scale_log2;  // scale > 0: the max commutes with it
+    const bool move = local > row_max + kRescaleLog2;
+    if (__any(move)) {
+      const float m_new = move ? local : row_max;
+      const float alpha = move ? __builtin_amdgcn_exp2f(row_max - m_new) : 1.f;
+#pragma unroll
+      for (int db = 0; db < 9; ++db) acc[db] *= alpha;
+      row_max = m_new;
+    }
+    const float ref = row_max == -INFINITY ? INFINITY : row_max;  // nothing yet: weights 0
+    X4 pb;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      pb[i] = static_cast<T>(__builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale_log2, -ref)));
+    }
+    if (left > 1) {  // V(c): what was issued behind it may be in flight
+      wait_vmcnt<12>();
+    } else if (left == 1) {
+      wait_vmcnt<8>();
+    } else {
+      wait_vmcnt<0>();
+    }
+    const u32x4* const v_tile = ring + (3 + (c & 1)) * 256;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+      acc[db] = E::mfma16(__builtin_bit_cast(X4, v_tr_read(v_tile, tr_key, 16 * db + tr_dim)), pb, acc[db]);
+    }
+    acc[8] = E::mfma16(ones, pb, acc[8]);
+    now = ahead1;
+    ahead1 = ahead2;
+    slot = slot == 2 ? 0 : slot + 1;
+  }
+  if (c16 < group) {
+    float* dst = part_acc + c16 * kDim + 4 * g4;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(dst + 16 * db) = acc[db];
+    if (g4 == 0) part_ml[c16] = f32x2{row_max, acc[8][0]};
+  }
+}
+
 struct SharedArgs {
   const uint16_t* q;
   const uint8_t* key_cache;
@@ -754,12 +920,19 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   __shared__ TileShared sh;
   const const_i32* const plan = (const const_i32*)a.plan;
   if (!plan_fits(plan, a.num_seqs, a.num_groups, a.num_kv_heads, a.group)) return;
-  const int32_t entry = static_cast<int32_t>(blockIdx.x / static_cast<uint32_t>(a.num_kv_heads));
-  const int32_t turn = static_cast<int32_t>(blockIdx.x) - entry * a.num_kv_heads;
-  // The kv head rotates with the entry, so that no XCD (workgroup id % 8)
-  // stays on one byte offset of the rows.
+  // Workgroups of the prefix's entries, one per kv head each; then one per
+  // four (rest entry, kv head) items.  The kv head rotates with the entry, so
+  // that no XCD (workgroup id % 8) stays on one byte offset of the rows.
+  const int64_t prefix_groups = a.shape.prefix * a.num_kv_heads;
+  const bool is_prefix = blockIdx.x < prefix_groups;
+  int64_t item = blockIdx.x;
+  if (!is_prefix) {
+    item = 4 * (item - prefix_groups) + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  }
+  const int32_t entry = static_cast<int32_t>(item / a.num_kv_heads);
+  const int32_t turn = static_cast<int32_t>(item - static_cast<int64_t>(entry) * a.num_kv_heads);
   const int32_t period = 8 / min(8, a.num_kv_heads & -a.num_kv_heads);
-  const int32_t kh = (turn + entry / period) % a.num_kv_heads;
+  const int32_t kh = (turn + (is_prefix ? entry / period : 4 * (entry & 0xFFFF))) % a.num_kv_heads;
   KeySource src;
   src.k_head = a.key_cache + static_cast<int64_t>(kh) * (kDim * 2);
   src.v_head = a.value_cache + static_cast<int64_t>(kh) * (kDim * 2);
@@ -773,7 +946,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   rows.q = a.q + static_cast<int64_t>(kh) * a.group * kDim;
   rows.seq_stride = a.q_seq_stride;
   rows.group = a.group;
-  if (entry < a.shape.prefix) {
+  if (is_prefix) {
     const const_i32* const e = plan + 4 * (a.shape.prefix_at() + 2 * entry);
     const int32_t log2 = e[3];
     rows.first = e[0];
@@ -804,19 +977,18 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     }
     return;
   }
-  const int32_t s = entry - static_cast<int32_t>(a.shape.prefix);
-  const const_i32* const e = plan + 4 * (a.shape.rest_at() + s);
-  rows.first = e[0];
-  rows.row0 = 0;
-  rows.rows = a.group;
+  if (entry >= a.shape.rest) return;
+  const const_i32* const e = plan + 4 * (a.shape.rest_at() + entry);
+  const int32_t seq = e[0];
   src.begin = e[1];
   src.end = e[2];
   src.stream = true;
-  if (rows.first < 0 || rows.first >= a.num_seqs || src.begin < 0 || src.end <= src.begin) return;
-  src.table = (const const_i32*)(a.tables + static_cast<int64_t>(rows.first) * a.table_stride);
+  if (seq < 0 || seq >= a.num_seqs || src.begin < 0 || src.end <= src.begin) return;
+  src.table = (const const_i32*)(a.tables + static_cast<int64_t>(seq) * a.table_stride);
   const int64_t row = a.num_kv_heads * a.shape.prefix_rows +
-                      (static_cast<int64_t>(s) * a.num_kv_heads + kh) * a.group;
-  attend<1, 1, kChunked, kHalf>(sh, src, rows, a.scale_log2, a.part_acc + row * kDim, a.part_ml + row);
+                      (static_cast<int64_t>(entry) * a.num_kv_heads + kh) * a.group;
+  attend_solo<kChunked, kHalf>(sh, src, rows.q + seq * a.q_seq_stride, a.group, a.scale_log2,
+                               a.part_acc + row * kDim, a.part_ml + row);
 }
 
 // Adds up the partials of (sequence, query head) pairs: those of the prefix's
@@ -1023,7 +1195,7 @@ extern "C" int nkv_shared_prefix_attention_decode(
     return nkv_fail(NKV_E_INVALID,
                     "%s: q/caches/plan/workspace must be 16-byte aligned and out rows 4-byte aligned", what);
   }
-  const int64_t items = (shape.prefix + shape.rest) * num_kv_heads;
+  const int64_t items = shape.prefix * num_kv_heads + (shape.rest * num_kv_heads + 3) / 4;
   const int64_t pairs = num_seqs * num_q_heads;
   if (items > INT32_MAX || pairs > INT32_MAX) {
     return nkv_fail(NKV_E_INVALID, "%s: too many sequences and heads for one launch", what);
