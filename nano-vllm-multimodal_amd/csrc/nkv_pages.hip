@@ -17,7 +17,7 @@ constexpr int kCopyBytes = 4096;  // per workgroup
 template <int W>
 __global__ __launch_bounds__(kCopyThreads) void copy_blocks_kernel(
     const uint8_t* __restrict__ src, uint8_t* __restrict__ dst, int64_t src_blocks, int64_t dst_blocks,
-    int64_t block_bytes, int32_t pieces, const int2* __restrict__ pairs) {
+    int64_t block_bytes, int32_t pieces, const int2* __restrict__ pairs, int32_t num_pairs) {
   typedef typename Word<W>::type T;
   const int32_t pair = static_cast<int32_t>(blockIdx.x) / pieces;
   const int32_t piece = static_cast<int32_t>(blockIdx.x) - pair * pieces;
@@ -29,15 +29,23 @@ __global__ __launch_bounds__(kCopyThreads) void copy_blocks_kernel(
   const int32_t words = static_cast<int32_t>(min(static_cast<int64_t>(kCopyBytes), block_bytes - begin) / W);
   const T* from = reinterpret_cast<const T*>(src + (plane * src_blocks + p.x) * block_bytes + begin);
   T* to = reinterpret_cast<T*>(dst + (plane * dst_blocks + p.y) * block_bytes + begin);
-  for (int32_t w = threadIdx.x; w < words; w += kCopyThreads) store_stream(to + w, load_stream(from + w));
+  // A page copied to several places (the samples of one prompt) is read
+  // through the caches: its copies lie next to each other in the list.
+  const bool again = (pair > 0 && pairs[pair - 1].x == p.x) || (pair + 1 < num_pairs && pairs[pair + 1].x == p.x);
+  if (again) {
+    for (int32_t w = threadIdx.x; w < words; w += kCopyThreads) store_stream(to + w, from[w]);
+  } else {
+    for (int32_t w = threadIdx.x; w < words; w += kCopyThreads) store_stream(to + w, load_stream(from + w));
+  }
 }
 
 template <int W>
 void launch_copy(dim3 grid, hipStream_t s, const void* src, void* dst, int64_t src_blocks,
-                 int64_t dst_blocks, int64_t block_bytes, int32_t pieces, const int32_t* pairs) {
+                 int64_t dst_blocks, int64_t block_bytes, int32_t pieces, const int32_t* pairs,
+                 int64_t num_pairs) {
   copy_blocks_kernel<W><<<grid, dim3(kCopyThreads), 0, s>>>(
       static_cast<const uint8_t*>(src), static_cast<uint8_t*>(dst), src_blocks, dst_blocks, block_bytes,
-      pieces, reinterpret_cast<const int2*>(pairs));
+      pieces, reinterpret_cast<const int2*>(pairs), static_cast<int32_t>(num_pairs));
 }
 
 }  // namespace
@@ -67,16 +75,16 @@ extern "C" int nkv_copy_blocks(const void* src, void* dst, int64_t planes, int64
   const auto n = static_cast<int32_t>(pieces);
   switch (w) {
     case 16:
-      launch_copy<16>(grid, s, src, dst, src_blocks, dst_blocks, block_bytes, n, pairs);
+      launch_copy<16>(grid, s, src, dst, src_blocks, dst_blocks, block_bytes, n, pairs, num_pairs);
       break;
     case 8:
-      launch_copy<8>(grid, s, src, dst, src_blocks, dst_blocks, block_bytes, n, pairs);
+      launch_copy<8>(grid, s, src, dst, src_blocks, dst_blocks, block_bytes, n, pairs, num_pairs);
       break;
     case 4:
-      launch_copy<4>(grid, s, src, dst, src_blocks, dst_blocks, block_bytes, n, pairs);
+      launch_copy<4>(grid, s, src, dst, src_blocks, dst_blocks, block_bytes, n, pairs, num_pairs);
       break;
     case 2:
-      launch_copy<2>(grid, s, src, dst, src_blocks, dst_blocks, block_bytes, n, pairs);
+      launch_copy<2>(grid, s, src, dst, src_blocks, dst_blocks, block_bytes, n, pairs, num_pairs);
       break;
     default:
       return nkv_fail(NKV_E_INVALID, "nkv_copy_blocks: caches and pages must be 2-byte aligned");

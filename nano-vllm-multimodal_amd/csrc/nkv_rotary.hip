@@ -37,7 +37,13 @@ struct Bf16 {
 struct Fp16 {
   typedef uint16_t T;
   static __device__ __forceinline__ float get(T v) { return static_cast<float>(__builtin_bit_cast(_Float16, v)); }
-  static __device__ __forceinline__ T put(float f) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f)); }
+  // The empty asm keeps the conversion apart from the fma before it: as one
+  // instruction it rounds once, and the compiler takes that in some forms of
+  // the kernel and not in others.
+  static __device__ __forceinline__ T put(float f) {
+    asm("" : "+v"(f));
+    return __builtin_bit_cast(uint16_t, static_cast<_Float16>(f));
+  }
 };
 struct Fp32 {
   typedef float T;
@@ -63,130 +69,172 @@ struct RotaryArgs {
   int64_t max_position, num_slots;
   int32_t num_tokens, q_heads, kv_heads, head_dim, half, wide_positions;
   int32_t section_end0, section_end1;  // first pairs of the second and third position row
-  int32_t heads_apart;                 // heads a thread's steps are apart
-  int32_t token_threads;               // threads per token
+  int32_t lanes;        // threads of a head
+  int32_t heads_apart;  // heads that a thread's are apart
+  int32_t block_tokens; // tokens of a workgroup
 };
+
+constexpr int kRotaryThreads = 256;
+constexpr int kRotaryHeads = 4;  // heads a thread handles at most in one go
+
+// Streaming accesses of a vector (16 bytes) or a single element.
+template <typename P>
+__device__ __forceinline__ P load_once(const P* p) {
+  if constexpr (sizeof(P) == 16) return __builtin_bit_cast(P, load_stream(reinterpret_cast<const u32x4*>(p)));
+  return *p;
+}
+template <typename P>
+__device__ __forceinline__ void store_once(P* p, const P& v) {
+  if constexpr (sizeof(P) == 16) {
+    store_stream(reinterpret_cast<u32x4*>(p), __builtin_bit_cast(u32x4, v));
+  } else {
+    *p = v;
+  }
+}
 
 // A thread handles two W-element vectors of a head: dims [W i, W i + W) and
 // the same past half (half layout), or 2 W dims in a row (interleaved): in
-// both the pairs [W i, W i + W), whose angles it loads once and keeps for
-// every head_apart-th head of its token.  Past the rotated dims its vectors
-// pass through.
+// both the pairs [W i, W i + W), whose angles it loads once and keeps for its
+// heads, every heads_apart-th of the token's q, k and (stored) v heads.  Past
+// the rotated dims its vectors pass through.
 template <typename E, int W, bool kInterleaved, bool kStore>
-__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
+__global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   typedef typename E::T T;
-  typedef T Vec __attribute__((ext_vector_type(W)));
   struct alignas(sizeof(T) * W) Pack {
     T e[W];
   };
-  const int64_t thread = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int32_t token = static_cast<int32_t>(thread / a.token_threads);
-  if (token >= a.num_tokens) return;
-  const int32_t rest = static_cast<int32_t>(thread - static_cast<int64_t>(token) * a.token_threads);
-  const int32_t lanes = (a.head_dim + 2 * W - 1) / (2 * W);  // threads of a head
-  const int32_t h0 = rest / lanes;
-  const int32_t lane = rest - h0 * lanes;
+  const int32_t token_threads = a.lanes * a.heads_apart;
+  // (Heads of more than kRotaryThreads lanes: one workgroup for each so many.)
+  const int32_t in_block = a.lanes > kRotaryThreads ? 0 : static_cast<int32_t>(threadIdx.x) / token_threads;
+  const int32_t rest = static_cast<int32_t>(threadIdx.x) - in_block * token_threads;
+  const int64_t token = static_cast<int64_t>(blockIdx.x) * a.block_tokens + in_block;
+  const int32_t h0 = a.lanes > kRotaryThreads ? 0 : rest / a.lanes;
+  const int32_t lane = a.lanes > kRotaryThreads
+                           ? static_cast<int32_t>(blockIdx.y * kRotaryThreads + threadIdx.x)
+                           : rest - h0 * a.lanes;
+  if (in_block >= a.block_tokens || token >= a.num_tokens || lane >= a.lanes) return;
   const int32_t j0 = lane * W;  // first pair, when rotated
   const bool rotated = j0 < a.half;
   const int32_t at1 = kInterleaved || !rotated ? 2 * j0 : j0;
   const int32_t at2 = kInterleaved || !rotated ? 2 * j0 + W : j0 + a.half;
   const bool both = at2 < a.head_dim;  // (an odd dim at the end, W == 1)
+  const int32_t heads = a.q_heads + (kStore ? 2 : 1) * a.kv_heads;
 
-  // The token's position of pair j.
-  auto position_of = [&](int32_t j) -> int64_t {
-    const int64_t row = a.position_row == 0 || j < a.section_end0 ? 0 : j < a.section_end1 ? 1 : 2;
-    const int64_t at = row * a.position_row + token;
-    return a.wide_positions ? static_cast<const int64_t*>(a.positions)[at]
-                            : static_cast<const int32_t*>(a.positions)[at];
-  };
-  float cosine[W], sine[W];
-  bool known = true;  // every position of the token is in the table
-  {
-    const int32_t rows = a.position_row == 0 ? 1 : 3;
-    for (int32_t r = 0; r < rows; ++r) {
-      const int64_t p = a.wide_positions
-                            ? static_cast<const int64_t*>(a.positions)[r * a.position_row + token]
-                            : static_cast<const int32_t*>(a.positions)[r * a.position_row + token];
-      known = known && p >= 0 && p < a.max_position;
-    }
-  }
+  int64_t position[3];
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    cosine[w] = 1.f;
-    sine[w] = 0.f;
-  }
-  if (rotated && known) {
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float2 cs = a.table[position_of(j0 + w) * a.half + j0 + w];
-      cosine[w] = cs.x;
-      sine[w] = cs.y;
-    }
+  for (int r = 0; r < 3; ++r) {
+    const int64_t at = r * a.position_row + token;
+    position[r] = a.wide_positions ? static_cast<const int64_t*>(a.positions)[at]
+                                   : static_cast<const int32_t*>(a.positions)[at];
   }
   int64_t slot = -1;
-  if (kStore) {
-    slot = a.slots[token];
-    if (slot >= a.num_slots || !known) slot = -1;
-  }
+  if (kStore) slot = a.slots[token];
+  // The first heads' vectors are on their way while the angles are looked up.
+  Pack x[kRotaryHeads], y[kRotaryHeads];
+  auto load = [&](int32_t first) {
+#pragma unroll
+    for (int i = 0; i < kRotaryHeads; ++i) {
+      const int32_t h = first + i * a.heads_apart;
+      if (h < heads) {
+        const int32_t kh = h - a.q_heads, vh = kh - a.kv_heads;
+        const bool is_v = kStore && vh >= 0;
+        const T* const src = kh < 0  ? static_cast<const T*>(a.q) + token * a.q_token + h * a.q_head
+                             : is_v ? static_cast<const T*>(a.v) + token * a.v_token + vh * a.v_head
+                                    : static_cast<const T*>(a.k) + token * a.k_token + kh * a.k_head;
+        x[i] = load_once(reinterpret_cast<const Pack*>(src + (is_v ? 2 * j0 : at1)));
+        if (is_v ? 2 * j0 + W < a.head_dim : both) {
+          y[i] = load_once(reinterpret_cast<const Pack*>(src + (is_v ? 2 * j0 + W : at2)));
+        }
+      }
+    }
+  };
+  load(h0);
 
-  const int32_t heads = a.q_heads + (kStore ? 2 : 1) * a.kv_heads;
-  for (int32_t h = h0; h < heads; h += a.heads_apart) {
-    const bool is_q = h < a.q_heads;
-    const int32_t kh = h - a.q_heads;
-    const bool is_v = kStore && kh >= a.kv_heads;
-    if (is_v) {
-      if (slot < 0) continue;
-      const int32_t vh = kh - a.kv_heads;
-      const T* src = static_cast<const T*>(a.v) + token * a.v_token + vh * a.v_head;
-      T* dst = static_cast<T*>(a.value_cache) + (slot * a.kv_heads + vh) * a.head_dim;
-      *reinterpret_cast<Pack*>(dst + 2 * j0) = *reinterpret_cast<const Pack*>(src + 2 * j0);
-      if (2 * j0 + W < a.head_dim) {
-        *reinterpret_cast<Pack*>(dst + 2 * j0 + W) = *reinterpret_cast<const Pack*>(src + 2 * j0 + W);
+  const bool known = position[0] >= 0 && position[0] < a.max_position && position[1] >= 0 &&
+                     position[1] < a.max_position && position[2] >= 0 && position[2] < a.max_position;
+  float cosine[W], sine[W];
+  if (rotated && known) {
+    auto row_of = [&](int32_t j) { return j < a.section_end0 ? 0 : j < a.section_end1 ? 1 : 2; };
+    auto entry = [&](int32_t j) {
+      const int row = row_of(j);
+      const int64_t p = row == 0 ? position[0] : row == 1 ? position[1] : position[2];
+      return a.table + p * a.half + j;
+    };
+    if (W > 1 && row_of(j0) == row_of(j0 + W - 1)) {  // one position: 16 bytes at a time
+      const float4* const from = reinterpret_cast<const float4*>(entry(j0));
+#pragma unroll
+      for (int w = 0; w < W / 2; ++w) {
+        const float4 cs = from[w];
+        cosine[2 * w] = cs.x;
+        sine[2 * w] = cs.y;
+        cosine[(2 * w + 1) % W] = cs.z;
+        sine[(2 * w + 1) % W] = cs.w;
       }
-      continue;
-    }
-    const T* src = is_q ? static_cast<const T*>(a.q) + token * a.q_token + h * a.q_head
-                        : static_cast<const T*>(a.k) + token * a.k_token + kh * a.k_head;
-    Pack x = *reinterpret_cast<const Pack*>(src + at1), y{};
-    if (both) y = *reinterpret_cast<const Pack*>(src + at2);
-    if (!known) {
-      x = Pack{};
-      y = Pack{};
-    } else if (rotated) {
-      float f[2 * W];
+    } else {
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        f[w] = E::get(x.e[w]);
-        f[W + w] = E::get(y.e[w]);
+        const float2 cs = *entry(j0 + w);
+        cosine[w] = cs.x;
+        sine[w] = cs.y;
       }
+    }
+  }
+  if (slot >= a.num_slots || !known) slot = -1;
+
+  for (int32_t first = h0; first < heads; first += kRotaryHeads * a.heads_apart) {
+    if (first != h0) load(first);
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const int i1 = kInterleaved ? 2 * w : w, i2 = kInterleaved ? 2 * w + 1 : W + w;
-        const float x1 = f[i1], x2 = f[i2];
-        f[i1] = x1 * cosine[w] - x2 * sine[w];
-        f[i2] = x2 * cosine[w] + x1 * sine[w];
+    for (int i = 0; i < kRotaryHeads; ++i) {
+      const int32_t h = first + i * a.heads_apart;
+      if (h >= heads) continue;
+      const int32_t kh = h - a.q_heads, vh = kh - a.kv_heads;
+      if (kStore && vh >= 0) {
+        if (slot < 0) continue;
+        T* const dst = static_cast<T*>(a.value_cache) + (slot * a.kv_heads + vh) * a.head_dim + 2 * j0;
+        store_once(reinterpret_cast<Pack*>(dst), x[i]);
+        if (2 * j0 + W < a.head_dim) store_once(reinterpret_cast<Pack*>(dst + W), y[i]);
+        continue;
       }
+      if (!known) {
+        x[i] = Pack{};
+        y[i] = Pack{};
+      } else if (rotated) {
+        float f[2 * W];
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        x.e[w] = E::put(f[w]);
-        y.e[w] = E::put(f[W + w]);
+        for (int w = 0; w < W; ++w) {
+          f[w] = E::get(x[i].e[w]);
+          f[W + w] = E::get(y[i].e[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          const int i1 = kInterleaved ? 2 * w : w, i2 = kInterleaved ? 2 * w + 1 : W + w;
+          const float x1 = f[i1], x2 = f[i2];
+          // Fused alike in every form, so that all give the same bits.
+          f[i1] = __builtin_fmaf(x1, cosine[w], -(x2 * sine[w]));
+          f[i2] = __builtin_fmaf(x2, cosine[w], x1 * sine[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+          x[i].e[w] = E::put(f[w]);
+          y[i].e[w] = E::put(f[W + w]);
+        }
       }
-    }
-    if (is_q) {
-      T* dst = static_cast<T*>(a.q_out) + token * a.q_out_token + h * a.q_out_head;
-      *reinterpret_cast<Pack*>(dst + at1) = x;
-      if (both) *reinterpret_cast<Pack*>(dst + at2) = y;
-      continue;
-    }
-    if (a.k_out != nullptr) {
-      T* dst = static_cast<T*>(a.k_out) + token * a.k_out_token + kh * a.k_out_head;
-      *reinterpret_cast<Pack*>(dst + at1) = x;
-      if (both) *reinterpret_cast<Pack*>(dst + at2) = y;
-    }
-    if (kStore && slot >= 0) {
-      T* dst = static_cast<T*>(a.key_cache) + (slot * a.kv_heads + kh) * a.head_dim;
-      *reinterpret_cast<Pack*>(dst + at1) = x;
-      if (both) *reinterpret_cast<Pack*>(dst + at2) = y;
+      if (kh < 0) {
+        T* const dst = static_cast<T*>(a.q_out) + token * a.q_out_token + h * a.q_out_head;
+        *reinterpret_cast<Pack*>(dst + at1) = x[i];
+        if (both) *reinterpret_cast<Pack*>(dst + at2) = y[i];
+        continue;
+      }
+      if (a.k_out != nullptr) {
+        T* const dst = static_cast<T*>(a.k_out) + token * a.k_out_token + kh * a.k_out_head;
+        *reinterpret_cast<Pack*>(dst + at1) = x[i];
+        if (both) *reinterpret_cast<Pack*>(dst + at2) = y[i];
+      }
+      if (kStore && slot >= 0) {
+        T* const dst = static_cast<T*>(a.key_cache) + (slot * a.kv_heads + kh) * a.head_dim;
+        store_once(reinterpret_cast<Pack*>(dst + at1), x[i]);
+        if (both) store_once(reinterpret_cast<Pack*>(dst + at2), y[i]);
+      }
     }
   }
 }
@@ -292,10 +340,15 @@ extern "C" int nkv_rotary(const nkv_rotary_desc* d, void* stream) {
   const int64_t w = wide ? static_cast<int64_t>(vec) : 1;
   const int64_t lanes = (d->head_dim + 2 * w - 1) / (2 * w);
   const int64_t heads = d->num_q_heads + (store ? 2 : 1) * d->num_kv_heads;
-  int64_t apart = heads;
-  while (apart > 8 && d->num_tokens * lanes * apart > 256 * 2048) apart = (apart + 1) / 2;
-  const int64_t threads = lanes * apart;
-  const int64_t blocks = (d->num_tokens * threads + 255) / 256;
+  // Heads per thread: one, until that alone would fill the chip, then up to
+  // kRotaryHeads, which share their angles and are in flight together.
+  int64_t each = d->num_tokens * lanes * heads / (256 * 2048);
+  each = each < 1 ? 1 : each > kRotaryHeads ? kRotaryHeads : each;
+  int64_t apart = (heads + each - 1) / each;
+  if (apart * lanes > kRotaryThreads) apart = lanes < kRotaryThreads ? kRotaryThreads / lanes : 1;
+  const int64_t block_tokens = lanes < kRotaryThreads ? kRotaryThreads / (lanes * apart) : 1;
+  const int64_t blocks = (d->num_tokens + block_tokens - 1) / block_tokens;
+  const int64_t lane_blocks = (lanes + kRotaryThreads - 1) / kRotaryThreads;
   if (blocks > INT32_MAX) return nkv_fail(NKV_E_INVALID, "nkv_rotary: too many tokens for one launch");
   RotaryArgs a{};
   a.q = d->q;
@@ -329,8 +382,9 @@ extern "C" int nkv_rotary(const nkv_rotary_desc* d, void* stream) {
   a.wide_positions = d->position_bytes == 8 ? 1 : 0;
   a.section_end0 = static_cast<int32_t>(d->section_ends[0]);
   a.section_end1 = static_cast<int32_t>(d->section_ends[1]);
+  a.lanes = static_cast<int32_t>(lanes);
   a.heads_apart = static_cast<int32_t>(apart);
-  a.token_threads = static_cast<int32_t>(threads);
+  a.block_tokens = static_cast<int32_t>(block_tokens);
   const bool inter = d->layout == NKV_ROTARY_INTERLEAVED;
   void (*kernel)(RotaryArgs) = nullptr;
   if (d->dtype == NKV_DTYPE_FLOAT32) {
@@ -340,6 +394,6 @@ extern "C" int nkv_rotary(const nkv_rotary_desc* d, void* stream) {
   } else {
     kernel = wide ? rotary_kernel_for<Bf16, 8>(inter, store) : rotary_kernel_for<Bf16, 1>(inter, store);
   }
-  kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<hipStream_t>(stream)>>>(a);
+  kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(lane_blocks)), dim3(kRotaryThreads), 0, static_cast<hipStream_t>(stream)>>>(a);
   return nkv_check_launch("nkv_rotary");
 }
