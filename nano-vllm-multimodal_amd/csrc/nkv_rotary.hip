@@ -11,6 +11,8 @@
 // at one radian per position has an fp32 spacing of 2^-7), so cosine and
 // sine come from a table built once in fp64, [max_position][rotary_dim / 2]
 // float2; a factor of the scaling multiplies both.
+#include <type_traits>
+
 #include "nkv_common.h"
 
 namespace nkv {
@@ -69,13 +71,10 @@ struct RotaryArgs {
   int64_t max_position, num_slots;
   int32_t num_tokens, q_heads, kv_heads, head_dim, half, wide_positions;
   int32_t section_end0, section_end1;  // first pairs of the second and third position row
-  int32_t lanes;        // threads of a head
-  int32_t heads_apart;  // heads that a thread's are apart
-  int32_t block_tokens; // tokens of a workgroup
+  int32_t lanes;  // threads of a head
 };
 
 constexpr int kRotaryThreads = 256;
-constexpr int kRotaryHeads = 4;  // heads a thread handles at most in one go
 
 // Streaming accesses of a vector (16 bytes) or a single element.
 template <typename P>
@@ -92,34 +91,48 @@ __device__ __forceinline__ void store_once(P* p, const P& v) {
   }
 }
 
-// A thread handles two W-element vectors of a head: dims [W i, W i + W) and
-// the same past half (half layout), or 2 W dims in a row (interleaved): in
-// both the pairs [W i, W i + W), whose angles it loads once and keeps for its
-// heads, every heads_apart-th of the token's q, k and (stored) v heads.  Past
-// the rotated dims its vectors pass through.
+// One thread per two W-element vectors of a head, of every q, k and (stored) v
+// head of a token.  Its vectors lie in the two halves of the rotated dims, of
+// the dims behind them, or of a v head, so that neighbouring threads move
+// neighbouring vectors: in the half layout they hold the two sides of W pairs,
+// in the interleaved one W / 2 pairs each (with 2 W dims in a row per thread
+// that form took 44.3 us where the half layout took 37.0, 8,192 tokens of 32 q
+// and 8 kv heads).
 template <typename E, int W, bool kInterleaved, bool kStore>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
   typedef typename E::T T;
   struct alignas(sizeof(T) * W) Pack {
     T e[W];
   };
-  const int32_t token_threads = a.lanes * a.heads_apart;
-  // (Heads of more than kRotaryThreads lanes: one workgroup for each so many.)
-  const int32_t in_block = a.lanes > kRotaryThreads ? 0 : static_cast<int32_t>(threadIdx.x) / token_threads;
-  const int32_t rest = static_cast<int32_t>(threadIdx.x) - in_block * token_threads;
-  const int64_t token = static_cast<int64_t>(blockIdx.x) * a.block_tokens + in_block;
-  const int32_t h0 = a.lanes > kRotaryThreads ? 0 : rest / a.lanes;
-  const int32_t lane = a.lanes > kRotaryThreads
-                           ? static_cast<int32_t>(blockIdx.y * kRotaryThreads + threadIdx.x)
-                           : rest - h0 * a.lanes;
-  if (in_block >= a.block_tokens || token >= a.num_tokens || lane >= a.lanes) return;
-  const int32_t j0 = lane * W;  // first pair, when rotated
-  const bool rotated = j0 < a.half;
-  const int32_t at1 = kInterleaved || !rotated ? 2 * j0 : j0;
-  const int32_t at2 = kInterleaved || !rotated ? 2 * j0 + W : j0 + a.half;
+  const uint32_t heads = a.q_heads + (kStore ? 2 : 1) * a.kv_heads;
+  const uint32_t thread = blockIdx.x * kRotaryThreads + threadIdx.x;  // below 2^31 (the launch)
+  const uint32_t head_of_all = thread / a.lanes;
+  const int32_t lane = static_cast<int32_t>(thread - head_of_all * a.lanes);
+  const int64_t token = head_of_all / heads;
+  const int32_t h = static_cast<int32_t>(head_of_all - static_cast<uint32_t>(token) * heads);
+  if (token >= a.num_tokens) return;
+  const int32_t kh = h - a.q_heads, vh = kh - a.kv_heads;
+  const bool is_v = kStore && vh >= 0;
+  const int32_t j0 = lane * W;
+  const bool rotated = j0 < a.half && !is_v;
+  int32_t at1, at2;
+  if (W == 1 && (kInterleaved || !rotated)) {  // single elements: two in a row
+    at1 = 2 * j0;
+    at2 = 2 * j0 + 1;
+  } else {
+    const int32_t begin = rotated || is_v ? 0 : a.half;  // in vectors' dims, of a half
+    const int32_t width = rotated ? a.half : is_v ? a.head_dim / 2 : a.head_dim / 2 - a.half;
+    at1 = 2 * begin + (j0 - begin);
+    at2 = at1 + width;
+  }
   const bool both = at2 < a.head_dim;  // (an odd dim at the end, W == 1)
-  const int32_t heads = a.q_heads + (kStore ? 2 : 1) * a.kv_heads;
 
+  // The vectors are on their way while the angles are looked up.
+  const T* const src = kh < 0  ? static_cast<const T*>(a.q) + token * a.q_token + h * a.q_head
+                       : is_v ? static_cast<const T*>(a.v) + token * a.v_token + vh * a.v_head
+                              : static_cast<const T*>(a.k) + token * a.k_token + kh * a.k_head;
+  Pack x = load_once(reinterpret_cast<const Pack*>(src + at1)), y{};
+  if (both) y = load_once(reinterpret_cast<const Pack*>(src + at2));
   int64_t position[3];
 #pragma unroll
   for (int r = 0; r < 3; ++r) {
@@ -128,31 +141,9 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
                                    : static_cast<const int32_t*>(a.positions)[at];
   }
   int64_t slot = -1;
-  if (kStore) slot = a.slots[token];
-  // The first heads' vectors are on their way while the angles are looked up.
-  Pack x[kRotaryHeads], y[kRotaryHeads];
-  auto load = [&](int32_t first) {
-#pragma unroll
-    for (int i = 0; i < kRotaryHeads; ++i) {
-      const int32_t h = first + i * a.heads_apart;
-      if (h < heads) {
-        const int32_t kh = h - a.q_heads, vh = kh - a.kv_heads;
-        const bool is_v = kStore && vh >= 0;
-        const T* const src = kh < 0  ? static_cast<const T*>(a.q) + token * a.q_token + h * a.q_head
-                             : is_v ? static_cast<const T*>(a.v) + token * a.v_token + vh * a.v_head
-                                    : static_cast<const T*>(a.k) + token * a.k_token + kh * a.k_head;
-        x[i] = load_once(reinterpret_cast<const Pack*>(src + (is_v ? 2 * j0 : at1)));
-        if (is_v ? 2 * j0 + W < a.head_dim : both) {
-          y[i] = load_once(reinterpret_cast<const Pack*>(src + (is_v ? 2 * j0 + W : at2)));
-        }
-      }
-    }
-  };
-  load(h0);
-
+  if (kStore && kh >= 0) slot = a.slots[token];
   const bool known = position[0] >= 0 && position[0] < a.max_position && position[1] >= 0 &&
                      position[1] < a.max_position && position[2] >= 0 && position[2] < a.max_position;
-  float cosine[W], sine[W];
   if (rotated && known) {
     auto row_of = [&](int32_t j) { return j < a.section_end0 ? 0 : j < a.section_end1 ? 1 : 2; };
     auto entry = [&](int32_t j) {
@@ -160,82 +151,79 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a) {
       const int64_t p = row == 0 ? position[0] : row == 1 ? position[1] : position[2];
       return a.table + p * a.half + j;
     };
-    if (W > 1 && row_of(j0) == row_of(j0 + W - 1)) {  // one position: 16 bytes at a time
-      const float4* const from = reinterpret_cast<const float4*>(entry(j0));
-#pragma unroll
-      for (int w = 0; w < W / 2; ++w) {
-        const float4 cs = from[w];
-        cosine[2 * w] = cs.x;
-        sine[2 * w] = cs.y;
-        cosine[(2 * w + 1) % W] = cs.z;
-        sine[(2 * w + 1) % W] = cs.w;
-      }
+    float cosine[W], sine[W];
+    if constexpr (W == 1) {
+      const float2 cs = *entry(j0);
+      cosine[0] = cs.x;
+      sine[0] = cs.y;
     } else {
+      constexpr int kSegments = kInterleaved ? 2 : 1;
+      constexpr int kPairs = W / kSegments;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float2 cs = *entry(j0 + w);
-        cosine[w] = cs.x;
-        sine[w] = cs.y;
+      for (int s = 0; s < kSegments; ++s) {  // W / 2 pairs, of the first and the second vector's (interleaved)
+        const int32_t j = kInterleaved ? (j0 + s * a.half) / 2 : j0;
+        float* const c = cosine + s * kPairs;
+        float* const d = sine + s * kPairs;
+        if (row_of(j) == row_of(j + kPairs - 1)) {  // one position: 16 bytes at a time
+          const float4* const from = reinterpret_cast<const float4*>(entry(j));
+#pragma unroll
+          for (int w = 0; w < kPairs / 2; ++w) {
+            const float4 cs = from[w];
+            c[2 * w] = cs.x;
+            d[2 * w] = cs.y;
+            c[2 * w + 1] = cs.z;
+            d[2 * w + 1] = cs.w;
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < kPairs; ++w) {
+            const float2 cs = *entry(j + w);
+            c[w] = cs.x;
+            d[w] = cs.y;
+          }
+        }
       }
     }
+    float f[2 * W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      f[w] = E::get(x.e[w]);
+      f[W + w] = E::get(y.e[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const int i1 = kInterleaved ? 2 * w : w, i2 = kInterleaved ? 2 * w + 1 : W + w;
+      const float x1 = f[i1], x2 = f[i2];
+      // Fused alike in every form, so that all give the same bits.
+      f[i1] = __builtin_fmaf(x1, cosine[w], -(x2 * sine[w]));
+      f[i2] = __builtin_fmaf(x2, cosine[w], x1 * sine[w]);
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      x.e[w] = E::put(f[w]);
+      y.e[w] = E::put(f[W + w]);
+    }
+  } else if (!known) {
+    x = Pack{};
+    y = Pack{};
   }
-  if (slot >= a.num_slots || !known) slot = -1;
 
-  for (int32_t first = h0; first < heads; first += kRotaryHeads * a.heads_apart) {
-    if (first != h0) load(first);
-#pragma unroll
-    for (int i = 0; i < kRotaryHeads; ++i) {
-      const int32_t h = first + i * a.heads_apart;
-      if (h >= heads) continue;
-      const int32_t kh = h - a.q_heads, vh = kh - a.kv_heads;
-      if (kStore && vh >= 0) {
-        if (slot < 0) continue;
-        T* const dst = static_cast<T*>(a.value_cache) + (slot * a.kv_heads + vh) * a.head_dim + 2 * j0;
-        store_once(reinterpret_cast<Pack*>(dst), x[i]);
-        if (2 * j0 + W < a.head_dim) store_once(reinterpret_cast<Pack*>(dst + W), y[i]);
-        continue;
-      }
-      if (!known) {
-        x[i] = Pack{};
-        y[i] = Pack{};
-      } else if (rotated) {
-        float f[2 * W];
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          f[w] = E::get(x[i].e[w]);
-          f[W + w] = E::get(y[i].e[w]);
-        }
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const int i1 = kInterleaved ? 2 * w : w, i2 = kInterleaved ? 2 * w + 1 : W + w;
-          const float x1 = f[i1], x2 = f[i2];
-          // Fused alike in every form, so that all give the same bits.
-          f[i1] = __builtin_fmaf(x1, cosine[w], -(x2 * sine[w]));
-          f[i2] = __builtin_fmaf(x2, cosine[w], x1 * sine[w]);
-        }
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          x[i].e[w] = E::put(f[w]);
-          y[i].e[w] = E::put(f[W + w]);
-        }
-      }
-      if (kh < 0) {
-        T* const dst = static_cast<T*>(a.q_out) + token * a.q_out_token + h * a.q_out_head;
-        *reinterpret_cast<Pack*>(dst + at1) = x[i];
-        if (both) *reinterpret_cast<Pack*>(dst + at2) = y[i];
-        continue;
-      }
-      if (a.k_out != nullptr) {
-        T* const dst = static_cast<T*>(a.k_out) + token * a.k_out_token + kh * a.k_out_head;
-        *reinterpret_cast<Pack*>(dst + at1) = x[i];
-        if (both) *reinterpret_cast<Pack*>(dst + at2) = y[i];
-      }
-      if (kStore && slot >= 0) {
-        T* const dst = static_cast<T*>(a.key_cache) + (slot * a.kv_heads + kh) * a.head_dim;
-        store_once(reinterpret_cast<Pack*>(dst + at1), x[i]);
-        if (both) store_once(reinterpret_cast<Pack*>(dst + at2), y[i]);
-      }
-    }
+  if (kh < 0) {
+    T* const dst = static_cast<T*>(a.q_out) + token * a.q_out_token + h * a.q_out_head;
+    *reinterpret_cast<Pack*>(dst + at1) = x;
+    if (both) *reinterpret_cast<Pack*>(dst + at2) = y;
+    return;
+  }
+  if (!is_v && a.k_out != nullptr) {
+    T* const dst = static_cast<T*>(a.k_out) + token * a.k_out_token + kh * a.k_out_head;
+    *reinterpret_cast<Pack*>(dst + at1) = x;
+    if (both) *reinterpret_cast<Pack*>(dst + at2) = y;
+  }
+  if (kStore && slot >= 0 && slot < a.num_slots && known) {
+    T* const cache = static_cast<T*>(is_v ? a.value_cache : a.key_cache);
+    T* const dst = cache + (slot * a.kv_heads + (is_v ? vh : kh)) * a.head_dim;
+    store_once(reinterpret_cast<Pack*>(dst + at1), x);
+    if (both) store_once(reinterpret_cast<Pack*>(dst + at2), y);
   }
 }
 
@@ -340,16 +328,8 @@ extern "C" int nkv_rotary(const nkv_rotary_desc* d, void* stream) {
   const int64_t w = wide ? static_cast<int64_t>(vec) : 1;
   const int64_t lanes = (d->head_dim + 2 * w - 1) / (2 * w);
   const int64_t heads = d->num_q_heads + (store ? 2 : 1) * d->num_kv_heads;
-  // Heads per thread: one, until that alone would fill the chip, then up to
-  // kRotaryHeads, which share their angles and are in flight together.
-  int64_t each = d->num_tokens * lanes * heads / (256 * 2048);
-  each = each < 1 ? 1 : each > kRotaryHeads ? kRotaryHeads : each;
-  int64_t apart = (heads + each - 1) / each;
-  if (apart * lanes > kRotaryThreads) apart = lanes < kRotaryThreads ? kRotaryThreads / lanes : 1;
-  const int64_t block_tokens = lanes < kRotaryThreads ? kRotaryThreads / (lanes * apart) : 1;
-  const int64_t blocks = (d->num_tokens + block_tokens - 1) / block_tokens;
-  const int64_t lane_blocks = (lanes + kRotaryThreads - 1) / kRotaryThreads;
-  if (blocks > INT32_MAX) return nkv_fail(NKV_E_INVALID, "nkv_rotary: too many tokens for one launch");
+  // Threads are numbered in 31 bits: more tokens than that are several launches.
+  const int64_t most = INT32_MAX / (lanes * heads);
   RotaryArgs a{};
   a.q = d->q;
   a.k = d->k;
@@ -374,7 +354,6 @@ extern "C" int nkv_rotary(const nkv_rotary_desc* d, void* stream) {
   a.position_row = d->position_row_stride;
   a.max_position = d->max_position;
   a.num_slots = d->num_slots;
-  a.num_tokens = static_cast<int32_t>(d->num_tokens);
   a.q_heads = static_cast<int32_t>(d->num_q_heads);
   a.kv_heads = static_cast<int32_t>(d->num_kv_heads);
   a.head_dim = static_cast<int32_t>(d->head_dim);
@@ -383,8 +362,6 @@ extern "C" int nkv_rotary(const nkv_rotary_desc* d, void* stream) {
   a.section_end0 = static_cast<int32_t>(d->section_ends[0]);
   a.section_end1 = static_cast<int32_t>(d->section_ends[1]);
   a.lanes = static_cast<int32_t>(lanes);
-  a.heads_apart = static_cast<int32_t>(apart);
-  a.block_tokens = static_cast<int32_t>(block_tokens);
   const bool inter = d->layout == NKV_ROTARY_INTERLEAVED;
   void (*kernel)(RotaryArgs) = nullptr;
   if (d->dtype == NKV_DTYPE_FLOAT32) {
@@ -394,6 +371,22 @@ extern "C" int nkv_rotary(const nkv_rotary_desc* d, void* stream) {
   } else {
     kernel = wide ? rotary_kernel_for<Bf16, 8>(inter, store) : rotary_kernel_for<Bf16, 1>(inter, store);
   }
-  kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(lane_blocks)), dim3(kRotaryThreads), 0, static_cast<hipStream_t>(stream)>>>(a);
-  return nkv_check_launch("nkv_rotary");
+  auto advance = [](auto*& p, int64_t bytes) {
+    if (p != nullptr) p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(reinterpret_cast<uintptr_t>(p) + bytes);
+  };
+  for (int64_t done = 0; done < d->num_tokens; done += most) {
+    const int64_t tokens = d->num_tokens - done < most ? d->num_tokens - done : most;
+    a.num_tokens = static_cast<int32_t>(tokens);
+    const int64_t blocks = (tokens * heads * lanes + kRotaryThreads - 1) / kRotaryThreads;
+    kernel<<<dim3(static_cast<unsigned>(blocks)), dim3(kRotaryThreads), 0, static_cast<hipStream_t>(stream)>>>(a);
+    if (int rc = nkv_check_launch("nkv_rotary")) return rc;
+    advance(a.q, most * a.q_token * eb);
+    advance(a.k, most * a.k_token * eb);
+    advance(a.v, most * a.v_token * eb);
+    advance(a.q_out, most * a.q_out_token * eb);
+    advance(a.k_out, most * a.k_out_token * eb);
+    advance(a.positions, most * d->position_bytes);
+    advance(a.slots, most * 4);
+  }
+  return NKV_OK;
 }
