@@ -572,8 +572,8 @@ int nkv_transfer_synchronize(nkv_transfer* lane);
  *                U, U + 1, ..., copies[first + k] = {old, new} and the
  *                number of moves goes to meta[5].
  *   Neither has a counterpart in the reference.  Both need
- *   nkv_pool_apply_copies, whose `copies` holds max_copies int32 pairs; the
- *   pages themselves are moved by nkv_copy_blocks.  A FORK's pair is only
+ *   nkv_pool_apply_copies, whose `copies` holds max_copies int32 pairs (those
+ *   that no op writes become {-1, -1}); the pages themselves are moved by nkv_copy_blocks.  A FORK's pair is only
  *   good until a later op frees its source.
  *   Consecutive APPENDs, and consecutive ALLOCATEs without cached ids, run
  *   as one parallel step up to the first repeated slot; the result is the

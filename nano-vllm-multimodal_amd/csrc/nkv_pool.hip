@@ -307,6 +307,8 @@ __global__ __launch_bounds__(kPoolThreads) void pool_apply_kernel(
   Cursor c{v.meta[0], v.meta[1], v.meta[2]};
   int32_t err = 0;
   int64_t err_op = 0;
+  // Pairs that no op writes (a failed log's) copy nothing.
+  for (int64_t i = t; i < max_copies; i += kPoolThreads) copies[i] = make_int2(-1, -1);
   if (v.meta[4] != 0) return;  // an earlier log failed: the pool stays as it was
 
   int64_t i = 0;

@@ -201,7 +201,7 @@ class DeviceBlockPool:
         nanokv.benchmark.LaunchTimer) brackets the apply kernel alone."""
         if not self._ops:
             return
-        copies = torch.full((self._pairs, 2), -1, dtype=torch.int32, device=self.device)
+        copies = torch.empty((self._pairs, 2), dtype=torch.int32, device=self.device)
         self._flush(copies, timer)
         self.copies = copies
 
