@@ -77,7 +77,7 @@ typedef __attribute__((address_space(4))) const int32_t const_i32;
 //   two per sequence  {rest's first row, context length, first rest entry, rest entries}
 //                     {first entry of its group's first tile, pieces per tile, member, rows per tile}
 //   two per prefix entry  {first sequence, first query row, query rows, log2 of the rows its form holds}
-//                         {first key, past the last, rows per tile, whether the group has one tile}
+//                         {first key, past the last, rows per tile, 0}
 //   one per rest entry  {sequence, first row, past the last, 0}
 // Entries past the last of their kind are empty, so that a workgroup finds
 // its own at a fixed place, without the counts.
@@ -226,7 +226,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
     const int32_t k1 = min(rows, static_cast<int32_t>(static_cast<int64_t>(key_tiles) * (piece + 1) / pieces) * kTileKeys);
     plan[shape.prefix_at() + 2 * e] =
         make_int4(first, tile * tile_rows, tile_q, tile_log2(tile_q));
-    plan[shape.prefix_at() + 2 * e + 1] = make_int4(k0, k1, tile_rows, n * group <= tile_rows ? 1 : 0);
+    plan[shape.prefix_at() + 2 * e + 1] = make_int4(k0, k1, tile_rows, 0);
   }
   for (int32_t e = prefix_entries + t; e < shape.prefix; e += kPlanThreads) {
     plan[shape.prefix_at() + 2 * e] = make_int4(0, 0, 0, 0);
@@ -311,7 +311,6 @@ struct KeySource {
   uint32_t row_bytes;
   int32_t block_size, block_shift, num_blocks;
   int32_t begin, end;  // context rows; tiles start at begin rounded down to a chunk
-  bool stream;         // no other item reads these rows: the copies pass the caches by
 };
 
 // The item's query rows [row0, row0 + rows): row r is head r % group of the
@@ -326,6 +325,7 @@ struct RowSource {
 // the cache or the table: keys find their rows by lane reads, with no memory
 // access in the loop but where an item outgrows the window (blocks of 16
 // keys: every 1,024 keys).
+template <bool kChunked>
 struct BlockWindow {
   const KeySource& src;
   int32_t last, first, ids;
@@ -334,7 +334,7 @@ struct BlockWindow {
     last = block_at(src.end - 1);
   }
   __device__ __forceinline__ int32_t block_at(int32_t t) const {
-    return src.block_shift >= 0 ? t >> src.block_shift : t / src.block_size;
+    return kChunked ? t >> src.block_shift : t / src.block_size;
   }
   __device__ __forceinline__ void load(int32_t block) {
     first = block;
@@ -362,7 +362,8 @@ struct BlockWindow {
 // key 4 i + l / 16 to position l % 16 of its row.  Keys that are not there
 // (their bit in `there` is 0) copy zeros.  row: the cache row of the chunk's
 // first key, or, without whole chunks, of the lane's four keys.
-template <bool kChunked>
+// kStream: no other item reads these rows, the copies pass the caches by.
+template <bool kChunked, bool kStream>
 struct ChunkCopy {
   const KeySource& src;
   int c16, g4;
@@ -380,13 +381,8 @@ struct ChunkCopy {
     if (kChunked && there == 0xFFFFu) {
       const uint8_t* const base =
           scalar_pointer(head + static_cast<uint64_t>(static_cast<uint32_t>(row[0])) * src.row_bytes);
-      if (src.stream) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lds_copy16<true>(base, off[i], dst + i * 1024u);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) lds_copy16<false>(base, off[i], dst + i * 1024u);
-      }
+      for (int i = 0; i < 4; ++i) lds_copy16<kStream>(base, off[i], dst + i * 1024u);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -395,7 +391,7 @@ struct ChunkCopy {
         const int32_t at = kChunked ? row[0] + key : row[kChunked ? 0 : i];
         const uint8_t* const from =
             (there >> key) & 1u ? head + static_cast<uint64_t>(static_cast<uint32_t>(at)) * src.row_bytes : src.zeros;
-        lds_copy16<false>(from + place, dst + i * 1024u);
+        lds_copy16<kStream>(from + place, dst + i * 1024u);
       }
     }
   }
@@ -407,8 +403,8 @@ struct ChunkCopy {
   }
 };
 
-// kChunked: blocks are whole 16-key chunks (one block id per chunk, read as a
-// scalar); otherwise every key looks up its own.
+// kChunked: blocks are a power of two of keys, whole chunks (one block id per
+// chunk); otherwise every key looks up its own.
 template <int RW, int NMB, bool kChunked, bool kHalf>
 __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, const RowSource& rows,
                                        float scale_log2, float* __restrict__ part_acc,
@@ -446,7 +442,7 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
     }
   }
 
-  BlockWindow window(src);
+  BlockWindow<kChunked> window(src);
   // What is known of a tile from the copies of its K to its products: its
   // keys that are there (bit = key) and where this wavefront's chunk lies (a
   // cache row for its first key; without whole chunks a row for each of the
@@ -462,8 +458,7 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
       const int32_t t = tile_t + chunk * kChunk;
       const int32_t block = window.block_at(t);
       const int32_t id = __builtin_amdgcn_readlane(window.ids, (block - window.first) & (kWave - 1));
-      tile.row[0] = __builtin_amdgcn_readfirstlane(
-          t < src.end && id >= 0 ? id * src.block_size + (t - block * src.block_size) : 0);
+      tile.row[0] = (id << src.block_shift) + (t & (src.block_size - 1));
       tile.there = ~uint64_t{0};
       if (tile_t < src.begin || tile_t + kTileKeys > src.end || !window.ok) {
         tile.there = __ballot(window.row_of(tile_t + lane) >= 0);
@@ -476,7 +471,8 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
     }
     return tile;
   };
-  const ChunkCopy<kChunked> copy(src, lane);
+  // (A group of up to 64 rows is one tile: nothing else reads its keys.)
+  const ChunkCopy<kChunked, RW != 4> copy(src, lane);
   const uint32_t lds_k = lds_address(&sh.k[0][0]) + chunk * 4096u;
   const uint32_t lds_v = lds_address(&sh.v[0][0]) + chunk * 4096u;
 
@@ -782,7 +778,7 @@ __device__ __forceinline__ void attend_solo(TileShared& sh, const KeySource& src
       qb[dc] = __builtin_bit_cast(X8, v);
     }
   }
-  BlockWindow window(src);
+  BlockWindow<kChunked> window(src);
   const int32_t first_key = src.begin & ~(kChunk - 1);
   const int32_t chunks = (src.end - first_key + kChunk - 1) / kChunk;
   window.load(window.block_at(first_key));
@@ -798,7 +794,7 @@ __device__ __forceinline__ void attend_solo(TileShared& sh, const KeySource& src
       const int32_t id = __builtin_amdgcn_readlane(window.ids, (block - window.first) & (kWave - 1));
       const int32_t low = max(0, src.begin - t), high = min(kChunk, src.end - t);
       c.there = id >= 0 ? ((1u << high) - 1u) & ~((1u << low) - 1u) : 0u;
-      c.row[0] = __builtin_amdgcn_readfirstlane(id >= 0 ? id * src.block_size + (t - block * src.block_size) : 0);
+      c.row[0] = (id << src.block_shift) + (t & (src.block_size - 1));
     } else {
       const int32_t key = t + c16;
       const int32_t row = window.row_of(key);
@@ -808,7 +804,7 @@ __device__ __forceinline__ void attend_solo(TileShared& sh, const KeySource& src
     }
     return c;
   };
-  const ChunkCopy<kChunked> copy(src, lane);
+  const ChunkCopy<kChunked, true> copy(src, lane);
   const uint32_t lds_k = lds_address(reinterpret_cast<const u32x4*>(&sh)) + wave * kSoloBytes;
   const uint32_t lds_v = lds_k + 3 * 4096u;
   const u32x4* const ring = reinterpret_cast<const u32x4*>(&sh) + wave * (kSoloBytes / 16);
@@ -954,7 +950,6 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     rows.rows = e[2];
     src.begin = e[4];
     src.end = e[5];
-    src.stream = e[7] != 0;
     // Uniform exits for entries that name rows outside the batch.
     const int32_t tile_rows = e[6];
     const int64_t row = static_cast<int64_t>(entry) * tile_rows;
@@ -982,7 +977,6 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   const int32_t seq = e[0];
   src.begin = e[1];
   src.end = e[2];
-  src.stream = true;
   if (seq < 0 || seq >= a.num_seqs || src.begin < 0 || src.end <= src.begin) return;
   src.table = (const const_i32*)(a.tables + static_cast<int64_t>(seq) * a.table_stride);
   const int64_t row = a.num_kv_heads * a.shape.prefix_rows +
@@ -1220,7 +1214,7 @@ extern "C" int nkv_shared_prefix_attention_decode(
   a.num_groups = static_cast<int32_t>(num_groups);
   a.scale_log2 = scale * 1.4426950408889634f;  // log2(e)
   const bool half = dtype == NKV_DTYPE_FLOAT16;
-  const bool chunked = block_size % kChunk == 0;
+  const bool chunked = block_size % kChunk == 0 && a.block_shift >= 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   void (*kernel)(SharedArgs) =
       chunked ? (half ? shared_attention_kernel<true, true> : shared_attention_kernel<true, false>)
