@@ -53,6 +53,9 @@ constexpr int kSlots = 512;       // workgroups resident on the chip: two per CU
 #ifndef NKV_SHARED_REST_ROUNDS
 #define NKV_SHARED_REST_ROUNDS 4  // entries of the rests: about so many rounds of wavefronts
 #endif
+#ifndef NKV_SHARED_WIDE_PREFIX
+#define NKV_SHARED_WIDE_PREFIX 8
+#endif
 #ifndef NKV_SHARED_MIN_PREFIX
 #define NKV_SHARED_MIN_PREFIX 2  // shortest piece of a prefix, in 64-key tiles
 #endif
@@ -194,7 +197,9 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
   // kRestRounds rounds of wavefronts, within the plan's room for them.
   const int64_t slots = slots_per_head(num_kv_heads);
   const int64_t share = (prefix_units + rest_units / 4 + slots - 1) / slots;
-  const int64_t prefix_tiles = max(static_cast<int64_t>(kMinPrefixTiles), share);
+  const int64_t half = (2 * prefix_units + slots - 1) / slots;  // a workgroup per CU
+  const int64_t prefix_tiles = max(max(static_cast<int64_t>(kMinPrefixTiles), share),
+                                   min(half, static_cast<int64_t>(NKV_SHARED_WIDE_PREFIX)));
   const int64_t room = max(static_cast<int64_t>(1), shape.rest - num_seqs);
   const int64_t rest_chunks =
       max(max(static_cast<int64_t>(kMinRestChunks), rest_units / (4 * slots * kRestRounds) + 1),
@@ -719,9 +724,10 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
       if (g4 == 0) s_ml[wave * 32 + r] = f32x2{row_max[mb], acc[8][mb][0]};
     }
     __syncthreads();
-    const int total_rows = min(rows.rows, RW * NMB * 16);
-    for (int idx = tid; idx < total_rows * 32; idx += kThreads) {
-      const int row = idx >> 5, piece = idx & 31;
+#pragma unroll 4
+    for (int step = 0; step < RW * NMB * 16 * 32 / kThreads; ++step) {
+      const int row = (step * kThreads + tid) >> 5, piece = tid & 31;
+      if (row >= rows.rows) continue;
       const int from = row / 32, r = row & 31;  // row wave and its row
       float top = -INFINITY;
 #pragma unroll
@@ -908,14 +914,16 @@ struct SharedArgs {
 // Whether the plan was built for this batch.
 __device__ __forceinline__ bool plan_fits(const const_i32* plan, int32_t num_seqs, int32_t num_groups,
                                           int32_t num_kv_heads, int32_t group) {
-  return plan[2] == num_seqs && plan[3] == num_groups && plan[4] == num_kv_heads && plan[5] == group;
+  return ((plan[2] ^ num_seqs) | (plan[3] ^ num_groups) | (plan[4] ^ num_kv_heads) | (plan[5] ^ group)) == 0;
 }
 
 template <bool kChunked, bool kHalf>
 __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArgs a) {
   __shared__ TileShared sh;
   const const_i32* const plan = (const const_i32*)a.plan;
-  if (!plan_fits(plan, a.num_seqs, a.num_groups, a.num_kv_heads, a.group)) return;
+  // Another batch's plan leaves at the first use of an entry, below: the entry
+  // is on its way by then.
+  const bool fits = plan_fits(plan, a.num_seqs, a.num_groups, a.num_kv_heads, a.group);
   // Workgroups of the prefix's entries, one per kv head each; then one per
   // four (rest entry, kv head) items.  The kv head rotates with the entry, so
   // that no XCD (workgroup id % 8) stays on one byte offset of the rows.
@@ -953,7 +961,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
     // Uniform exits for entries that name rows outside the batch.
     const int32_t tile_rows = e[6];
     const int64_t row = static_cast<int64_t>(entry) * tile_rows;
-    if (rows.first < 0 || rows.row0 < 0 || rows.rows <= 0 || rows.rows > (1 << log2) || src.begin < 0 ||
+    if (!fits || rows.first < 0 || rows.row0 < 0 || rows.rows <= 0 || rows.rows > (1 << log2) || src.begin < 0 ||
         src.end <= src.begin || rows.rows > tile_rows || row + rows.rows > a.shape.prefix_rows ||
         rows.first + (static_cast<int64_t>(rows.row0) + rows.rows - 1) / a.group >= a.num_seqs) {
       return;
@@ -977,7 +985,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   const int32_t seq = e[0];
   src.begin = e[1];
   src.end = e[2];
-  if (seq < 0 || seq >= a.num_seqs || src.begin < 0 || src.end <= src.begin) return;
+  if (!fits || seq < 0 || seq >= a.num_seqs || src.begin < 0 || src.end <= src.begin) return;
   src.table = (const const_i32*)(a.tables + static_cast<int64_t>(seq) * a.table_stride);
   const int64_t row = a.num_kv_heads * a.shape.prefix_rows +
                       (static_cast<int64_t>(entry) * a.num_kv_heads + kh) * a.group;
@@ -1005,20 +1013,20 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a, uint16_
   const int32_t kh = qh / a.group, head = qh % a.group;
   uint32_t* const dst = reinterpret_cast<uint32_t*>(out + seq * out_seq_stride + qh * kDim + 2 * lane);
   const const_i32* const plan = (const const_i32*)a.plan;
+  const const_i32* const record = plan + 4 * (kPlanSeqs + 2 * static_cast<int64_t>(seq));
+  const int32_t rest_first = record[2], rest_count = record[3];
+  const int32_t prefix_entry = record[4], pieces = record[5], member = record[6];
+  const int32_t tile_rows = max(1, record[7]);
   if (!plan_fits(plan, a.num_seqs, a.num_groups, a.num_kv_heads, a.group)) {
     // Another batch's plan: no partial was written.  NaN, not stale values.
     if (part_wave == 0) *dst = kHalf ? 0x7E007E00u : 0x7FC07FC0u;
     return;
   }
-  const const_i32* const record = plan + 4 * (kPlanSeqs + 2 * static_cast<int64_t>(seq));
-  const int32_t rest_first = record[2], rest_count = record[3];
-  const int32_t pieces = record[5];
-  const int32_t row = record[6] * a.group + head;
-  const int32_t tile_rows = max(1, record[7]);
+  const int32_t row = member * a.group + head;
   const int32_t tile = row / tile_rows;
   // The row's first partial; its pieces lie tile_rows apart.
   const int64_t prefix_row = kh * a.shape.prefix_rows +
-                             (record[4] + static_cast<int64_t>(tile) * pieces) * tile_rows + row % tile_rows;
+                             (prefix_entry + static_cast<int64_t>(tile) * pieces) * tile_rows + row % tile_rows;
   const int64_t prefix_most = a.num_kv_heads * a.shape.prefix_rows - 1;
   const int64_t rest_row = a.num_kv_heads * a.shape.prefix_rows;
   const int32_t parts = pieces + rest_count;
