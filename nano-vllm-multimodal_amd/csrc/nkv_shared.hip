@@ -995,12 +995,16 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
 
 // Adds up the partials of (sequence, query head) pairs: those of the prefix's
 // pieces, then the rest's.  kWaves wavefronts per pair, each every kWaves-th
-// batch; a lane holds two dims.
-constexpr int kMergeBatch = 8;
+// batch; a lane holds two dims.  Few pairs leave the chip to the latency of a
+// wavefront's chain of batches: four share a pair then (call of 896 pairs 28.1
+// instead of 31.1 us, of 4,096 127.5 instead of 128.0; of 8,192 60.4 instead of
+// 56.0, of 32,768 190 instead of 181: there one wavefront each).
+constexpr int kMergePairs = 4096;  // up to so many pairs, four wavefronts each
 template <bool kHalf, int kWaves>
 __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a, uint16_t* __restrict__ out,
                                                            int64_t out_seq_stride) {
   constexpr int kPairs = 4 / kWaves;
+  constexpr int kMergeBatch = kWaves == 1 ? 8 : 4;
   const int lane = threadIdx.x & (kWave - 1);
   const int w4 = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int part_wave = w4 % kWaves;
@@ -1229,7 +1233,7 @@ extern "C" int nkv_shared_prefix_attention_decode(
               : (half ? shared_attention_kernel<false, true> : shared_attention_kernel<false, false>);
   kernel<<<dim3(static_cast<unsigned>(items)), dim3(kThreads), 0, s>>>(a);
   if (int rc = nkv_check_launch(what)) return rc;
-  const bool four = pairs <= 2048;
+  const bool four = pairs <= kMergePairs;
   void (*merge)(SharedArgs, uint16_t*, int64_t) =
       four ? (half ? shared_merge_kernel<true, 4> : shared_merge_kernel<false, 4>)
            : (half ? shared_merge_kernel<true, 1> : shared_merge_kernel<false, 1>);
