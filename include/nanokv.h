@@ -718,8 +718,9 @@ int nkv_rotary(const nkv_rotary_desc* desc, void* stream);
  * cu_groups[g+1]); the first prefix_lens[g] rows of their contexts are the
  * same (the same blocks, or the same contents) and are read through the
  * block table of the group's first sequence.  Groups of one sequence, groups
- * with no prefix, sequences in no group and sequences shorter than their
- * group's prefix share nothing and are read through their own tables.
+ * with no prefix, groups whose first sequence is shorter than it, sequences in
+ * no group and sequences shorter than their group's prefix share nothing and
+ * are read through their own tables.
  * Scores, weights' sums and outputs are held in fp32 and rounded once; the
  * weights are rounded to the input type before the product with V.
  * dtype, head_dim, heads, tables, q, out and scale as

@@ -14,20 +14,31 @@
 //
 // One launch holds both kinds of items, the prefix's first: they are bound
 // by the matrix cores, the others by HBM, so they run side by side on a CU.
-// An item is one workgroup of four wavefronts over 64-key tiles in LDS,
-// double-buffered and copied straight from the cache (global_load_lds).  RW
-// of its wavefronts split the query rows (32 each), 4 / RW the keys of a
-// tile; a group with few rows splits keys only, as does a sequence's rest
-// (16 rows: the query heads of a kv head), and then every wavefront reads
-// only the keys it copied itself, so its loop has no barrier.
+//   A prefix item is one workgroup of four wavefronts: up to 128 query rows of
+//     a kv head over 64-key tiles that all four read.  RW of them split the
+//     rows (32 each), 4 / RW the keys of a tile; up to 32 rows split keys
+//     only, and every wavefront reads only the keys it copied itself, with no
+//     barrier in its loop.
+//   A rest's item is one wavefront (attend_solo), four to a workgroup.
+// K and V go from the cache straight into rings of tiles in LDS
+// (global_load_lds), copies ahead of the products.
 //   S^T = K Q^T    16x16x32 MFMAs: a lane's scores belong to one query row
 //   O^T += V^T P^T the weights, rounded to the element type, straight from
 //                  the score registers; V^T from the transposing LDS read;
-//                  a product with ones sums the same rounded weights.
+//                  a product with ones sums the same rounded weights, so the
+//                  rounding of a weight (at most half a step of the type)
+//                  enters numerator and denominator alike.
 // Sequences shorter than their group's prefix share nothing and are read
-// from row 0 through their own table, so no row is masked inside a tile.
+// from row 0 through their own table, so no row is masked inside a tile; nor
+// does a group whose first sequence is, as its table would not hold the rows.
 // Keys in a block outside the cache or past the table are dropped: they copy
 // a row of zeros and their scores become -inf.
+//
+// 256 sequences of 16 query and 8 kv heads behind 16,384 shared keys, 16 to
+// 2,048 of their own (bf16, 533 MB, 35 GFLOP): 120 us; the rests alone 94 us,
+// 5.0 TB/s, the prefix alone 60 us.  Reading the prefix once per sequence
+// instead is 17.7 GB.  32 sequences of 28 and 4 heads behind 12,001 keys: 27
+// us, of which 21 are the attention; 8 sequences, 12 us, two launches' latency.
 #include <algorithm>
 #include <cmath>
 
@@ -44,27 +55,25 @@ constexpr int kChunk = 16;        // keys a wavefront copies per tile
 constexpr uint32_t kTileBytes = kTileKeys * 256;
 constexpr int kMaxGroup = 16;     // query heads per kv head
 constexpr int kTileRows = 128;    // query rows of a prefix tile at most
-constexpr int kMinTileRows = 32;  // ... and at least, where a group has more
-#ifndef NKV_SHARED_TILE_LOG2
-#define NKV_SHARED_TILE_LOG2 7
-#endif
 constexpr int kPlanThreads = 1024;
 constexpr int kSlots = 512;       // workgroups resident on the chip: two per CU
-#ifndef NKV_SHARED_REST_ROUNDS
-#define NKV_SHARED_REST_ROUNDS 4  // entries of the rests: about so many rounds of wavefronts
-#endif
-#ifndef NKV_SHARED_WIDE_PREFIX
-#define NKV_SHARED_WIDE_PREFIX 8
-#endif
-#ifndef NKV_SHARED_MIN_PREFIX
-#define NKV_SHARED_MIN_PREFIX 2  // shortest piece of a prefix, in 64-key tiles
-#endif
-#ifndef NKV_SHARED_MIN_REST
-#define NKV_SHARED_MIN_REST 4  // shortest entry of a rest, in 16-key chunks
-#endif
-constexpr int kRestRounds = NKV_SHARED_REST_ROUNDS;
-constexpr int kMinPrefixTiles = NKV_SHARED_MIN_PREFIX;
-constexpr int kMinRestChunks = NKV_SHARED_MIN_REST;
+// The rests' entries: about so many rounds of wavefronts over the chip, so
+// that the last round is a small part (the rests of 256 sequences 94.5 us; of
+// 8 rounds 98.2, of 2 94.6, and 124.7 instead of 124.0 beside a prefix), but
+// none shorter than kMinRestChunks chunks (13 groups of 96 sequences 46.3 us;
+// from 2 chunks on 50.3, from 8 on 47.0).
+constexpr int kRestRounds = 4;
+constexpr int kMinRestChunks = 4;
+// Pieces of a prefix, in 64-key tiles.  Those that could all run at once at
+// two workgroups per CU are cut for one per CU instead, up to kWidePieceTiles:
+// a piece of few tiles costs as much to start, to store its 128 rows of
+// partials and to merge them as to walk (28 heads over 12,001 keys 28.8 us,
+// cut for two 32.0; up to 12 and 16 tiles the same).  8 sequences behind
+// 1,511 keys take 12.6 us from 1 or 2 tiles on, 14.5 from 4.  Longer ones pay
+// for the second workgroup: it takes its weights while the first multiplies
+// (16,384 keys alone 60 us, cut for one 71).
+constexpr int kMinPieceTiles = 2;
+constexpr int kWidePieceTiles = 8;
 constexpr int32_t kMaxLength = 0x7FFFFF00;
 constexpr float kRescaleLog2 = 8.f;  // the reference max moves only past this
 
@@ -78,9 +87,9 @@ typedef __attribute__((address_space(4))) const int32_t const_i32;
 //   [1]  {num_kv_heads, query heads per kv head, 0, 0}
 //   [2, 18)  256 bytes of zeros, the row that dropped keys copy
 //   two per sequence  {rest's first row, context length, first rest entry, rest entries}
-//                     {first entry of its group's first tile, pieces per tile, member, rows per tile}
-//   two per prefix entry  {first sequence, first query row, query rows, log2 of the rows its form holds}
-//                         {first key, past the last, rows per tile, 0}
+//                     {first entry of its group's first tile, pieces per tile, member, 0}
+//   two per prefix entry  {first sequence, first query row, query rows, 0}
+//                         {first key, past the last, 0, 0}
 //   one per rest entry  {sequence, first row, past the last, 0}
 // Entries past the last of their kind are empty, so that a workgroup finds
 // its own at a fixed place, without the counts.
@@ -99,24 +108,20 @@ struct PlanShape {
 __host__ __device__ constexpr int64_t slots_per_head(int64_t kv_heads) {
   return kSlots / kv_heads > 0 ? kSlots / kv_heads : 1;
 }
-// With tiles of S query rows a plan has at most slots + (tiles) prefix
-// entries, at most sharing + rows / S tiles, whatever S it takes.
+// All pieces but a tile's last are full and a slot's share or longer: at most
+// slots + tiles prefix entries, and at most sharing + rows / kTileRows tiles.
 PlanShape plan_shape(int64_t num_seqs, int64_t num_groups, int64_t kv_heads, int64_t group,
                      int64_t rest_tokens) {
   PlanShape p{num_seqs, 0, 0, 0};
   const int64_t sharing = std::min(num_groups, num_seqs / 2);
   if (sharing > 0) {
-    p.prefix = slots_per_head(kv_heads) + sharing + num_seqs * group / kMinTileRows;
+    p.prefix = slots_per_head(kv_heads) + sharing + num_seqs * group / kTileRows;
     p.prefix_rows = (slots_per_head(kv_heads) + sharing) * kTileRows + num_seqs * group;
   }
   p.rest = 4 * slots_per_head(kv_heads) * kRestRounds;
   if (rest_tokens >= 0) p.rest = std::min(p.rest, rest_tokens / kChunk + 1);
   p.rest += num_seqs;
   return p;
-}
-
-__device__ __forceinline__ int32_t tile_log2(int64_t rows) {  // query rows per tile: 16, 32, 64 or 128
-  return rows <= 16 ? 4 : rows <= 32 ? 5 : rows <= 64 ? 6 : 7;
 }
 
 __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* s_sum) {
@@ -131,16 +136,22 @@ __device__ __forceinline__ int64_t block_sum(int64_t v, int64_t* s_sum) {
 }
 
 struct GroupOf {
+  const int32_t* cu_seqlens_k;
   const int32_t* cu;
   const int32_t* prefix;
   int32_t num_groups, num_seqs;
-  // A group that shares something: at least two sequences of the batch.
+  // (A key past the bound lies in no table; tile ends stay below 2^31.)
+  __device__ __forceinline__ int32_t length_of(int32_t i) const {
+    return min(max(0, cu_seqlens_k[i + 1] - cu_seqlens_k[i]), kMaxLength);
+  }
+  // A group that shares something: at least two sequences of the batch, the
+  // first of which, whose table the prefix is read through, has all of it.
   __device__ __forceinline__ bool shares(int32_t g, int32_t* first, int32_t* n, int32_t* rows) const {
     const int32_t s0 = cu[g], s1 = cu[g + 1];
     *first = s0;
     *n = s1 - s0;
     *rows = prefix[g];
-    return s0 >= 0 && s1 <= num_seqs && s1 - s0 >= 2 && *rows > 0 && *rows <= kMaxLength;
+    return s0 >= 0 && s1 <= num_seqs && s1 - s0 >= 2 && *rows > 0 && *rows <= length_of(s0);
   }
   // The group of sequence i, -1 for none.
   __device__ __forceinline__ int32_t of(int32_t i) const {
@@ -159,8 +170,7 @@ struct GroupOf {
 };
 
 __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
-    const int32_t* __restrict__ cu_seqlens_k, GroupOf groups, int32_t num_kv_heads, int32_t group,
-    PlanShape shape, int4* __restrict__ plan) {
+    GroupOf groups, int32_t num_kv_heads, int32_t group, PlanShape shape, int4* __restrict__ plan) {
   extern __shared__ int32_t s_mem[];
   __shared__ int64_t s_sum[kPlanThreads / kWave];
   __shared__ int32_t s_tmp[kPlanThreads / kWave + 1];
@@ -169,20 +179,18 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
   const int32_t num_groups = groups.num_groups;
   // Where sequence i's own part begins: its group's prefix, when it has all of it.
   auto rest_of = [&](int32_t i, int32_t* length) {
-    // (A key past the bound lies in no table; tile ends stay below 2^31.)
-    *length = min(max(0, cu_seqlens_k[i + 1] - cu_seqlens_k[i]), kMaxLength);
+    *length = groups.length_of(i);
     const int32_t g = groups.of(i);
     int32_t first, n, rows;
     return g >= 0 && groups.shares(g, &first, &n, &rows) && *length >= rows ? rows : 0;
   };
 
-  const int32_t tile_rows = 1 << NKV_SHARED_TILE_LOG2;
   int64_t prefix_units = 0, rest_units = 0;  // 64-key tiles and 16-key chunks to walk, per kv head
   for (int32_t g = t; g < num_groups; g += kPlanThreads) {
     int32_t first, n, rows;
     if (groups.shares(g, &first, &n, &rows)) {
       const int64_t q_rows = static_cast<int64_t>(n) * group;
-      const int64_t tiles = (q_rows + tile_rows - 1) / tile_rows;
+      const int64_t tiles = (q_rows + kTileRows - 1) / kTileRows;
       prefix_units += tiles * ((static_cast<int64_t>(rows) + kTileKeys - 1) / kTileKeys);
     }
   }
@@ -198,8 +206,8 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
   const int64_t slots = slots_per_head(num_kv_heads);
   const int64_t share = (prefix_units + rest_units / 4 + slots - 1) / slots;
   const int64_t half = (2 * prefix_units + slots - 1) / slots;  // a workgroup per CU
-  const int64_t prefix_tiles = max(max(static_cast<int64_t>(kMinPrefixTiles), share),
-                                   min(half, static_cast<int64_t>(NKV_SHARED_WIDE_PREFIX)));
+  const int64_t prefix_tiles = max(max(static_cast<int64_t>(kMinPieceTiles), share),
+                                   min(half, static_cast<int64_t>(kWidePieceTiles)));
   const int64_t room = max(static_cast<int64_t>(1), shape.rest - num_seqs);
   const int64_t rest_chunks =
       max(max(static_cast<int64_t>(kMinRestChunks), rest_units / (4 * slots * kRestRounds) + 1),
@@ -213,7 +221,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
       [&](int32_t g) {
         int32_t first, n, rows;
         if (!groups.shares(g, &first, &n, &rows)) return 0;
-        const int32_t tiles = (n * group + tile_rows - 1) / tile_rows;
+        const int32_t tiles = (n * group + kTileRows - 1) / kTileRows;
         return tiles * ((rows - 1) / piece_keys + 1);
       },
       s_mem, s_tmp);
@@ -224,14 +232,13 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
     groups.shares(g, &first, &n, &rows);
     const int32_t pieces = (rows - 1) / piece_keys + 1;
     const int32_t tile = (e - s_mem[g]) / pieces, piece = (e - s_mem[g]) % pieces;
-    const int32_t tile_q = min(tile_rows, n * group - tile * tile_rows);
+    const int32_t tile_q = min(kTileRows, n * group - tile * kTileRows);
     // Pieces of equal length, in whole tiles.
     const int32_t key_tiles = (rows - 1) / kTileKeys + 1;
     const int32_t k0 = static_cast<int32_t>(static_cast<int64_t>(key_tiles) * piece / pieces) * kTileKeys;
     const int32_t k1 = min(rows, static_cast<int32_t>(static_cast<int64_t>(key_tiles) * (piece + 1) / pieces) * kTileKeys);
-    plan[shape.prefix_at() + 2 * e] =
-        make_int4(first, tile * tile_rows, tile_q, tile_log2(tile_q));
-    plan[shape.prefix_at() + 2 * e + 1] = make_int4(k0, k1, tile_rows, 0);
+    plan[shape.prefix_at() + 2 * e] = make_int4(first, tile * kTileRows, tile_q, 0);
+    plan[shape.prefix_at() + 2 * e + 1] = make_int4(k0, k1, 0, 0);
   }
   for (int32_t e = prefix_entries + t; e < shape.prefix; e += kPlanThreads) {
     plan[shape.prefix_at() + 2 * e] = make_int4(0, 0, 0, 0);
@@ -243,7 +250,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
     int4 record = make_int4(0, 0, 0, 0);
     if (rest_of(i, &length) > 0) {
       groups.shares(g, &first, &n, &rows);
-      record = make_int4(s_mem[g], (rows - 1) / piece_keys + 1, i - first, tile_rows);
+      record = make_int4(s_mem[g], (rows - 1) / piece_keys + 1, i - first, 0);
     }
     plan[kPlanSeqs + 2 * i + 1] = record;
   }
@@ -952,28 +959,26 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   rows.group = a.group;
   if (is_prefix) {
     const const_i32* const e = plan + 4 * (a.shape.prefix_at() + 2 * entry);
-    const int32_t log2 = e[3];
     rows.first = e[0];
     rows.row0 = e[1];
     rows.rows = e[2];
     src.begin = e[4];
     src.end = e[5];
     // Uniform exits for entries that name rows outside the batch.
-    const int32_t tile_rows = e[6];
-    const int64_t row = static_cast<int64_t>(entry) * tile_rows;
-    if (!fits || rows.first < 0 || rows.row0 < 0 || rows.rows <= 0 || rows.rows > (1 << log2) || src.begin < 0 ||
-        src.end <= src.begin || rows.rows > tile_rows || row + rows.rows > a.shape.prefix_rows ||
+    const int64_t row = static_cast<int64_t>(entry) * kTileRows;
+    if (!fits || rows.first < 0 || rows.row0 < 0 || rows.rows <= 0 || rows.rows > kTileRows || src.begin < 0 ||
+        src.end <= src.begin || row + rows.rows > a.shape.prefix_rows ||
         rows.first + (static_cast<int64_t>(rows.row0) + rows.rows - 1) / a.group >= a.num_seqs) {
       return;
     }
     src.table = (const const_i32*)(a.tables + static_cast<int64_t>(rows.first) * a.table_stride);
     float* const acc = a.part_acc + (kh * a.shape.prefix_rows + row) * kDim;
     f32x2* const ml = a.part_ml + kh * a.shape.prefix_rows + row;
-    if (log2 >= 7) {
+    if (rows.rows > 64) {
       attend<4, 2, kChunked, kHalf>(sh, src, rows, a.scale_log2, acc, ml);
-    } else if (log2 == 6) {
+    } else if (rows.rows > 32) {
       attend<2, 2, kChunked, kHalf>(sh, src, rows, a.scale_log2, acc, ml);
-    } else if (log2 == 5) {
+    } else if (rows.rows > 16) {
       attend<1, 2, kChunked, kHalf>(sh, src, rows, a.scale_log2, acc, ml);
     } else {
       attend<1, 1, kChunked, kHalf>(sh, src, rows, a.scale_log2, acc, ml);
@@ -1020,22 +1025,21 @@ __global__ __launch_bounds__(256) void shared_merge_kernel(SharedArgs a, uint16_
   const const_i32* const record = plan + 4 * (kPlanSeqs + 2 * static_cast<int64_t>(seq));
   const int32_t rest_first = record[2], rest_count = record[3];
   const int32_t prefix_entry = record[4], pieces = record[5], member = record[6];
-  const int32_t tile_rows = max(1, record[7]);
   if (!plan_fits(plan, a.num_seqs, a.num_groups, a.num_kv_heads, a.group)) {
     // Another batch's plan: no partial was written.  NaN, not stale values.
     if (part_wave == 0) *dst = kHalf ? 0x7E007E00u : 0x7FC07FC0u;
     return;
   }
   const int32_t row = member * a.group + head;
-  const int32_t tile = row / tile_rows;
-  // The row's first partial; its pieces lie tile_rows apart.
+  const int32_t tile = row / kTileRows;
+  // The row's first partial; its pieces lie kTileRows apart.
   const int64_t prefix_row = kh * a.shape.prefix_rows +
-                             (prefix_entry + static_cast<int64_t>(tile) * pieces) * tile_rows + row % tile_rows;
+                             (prefix_entry + static_cast<int64_t>(tile) * pieces) * kTileRows + row % kTileRows;
   const int64_t prefix_most = a.num_kv_heads * a.shape.prefix_rows - 1;
   const int64_t rest_row = a.num_kv_heads * a.shape.prefix_rows;
   const int32_t parts = pieces + rest_count;
   auto row_of = [&](int32_t p) -> int64_t {
-    if (p < pieces) return min(prefix_row + static_cast<int64_t>(p) * tile_rows, prefix_most);
+    if (p < pieces) return min(prefix_row + static_cast<int64_t>(p) * kTileRows, prefix_most);
     const int64_t e = min(static_cast<int64_t>(rest_first) + p - pieces, a.shape.rest - 1);
     return rest_row + (e * a.num_kv_heads + kh) * a.group + head;
   };
@@ -1145,11 +1149,11 @@ extern "C" int nkv_build_shared_plan(const int32_t* cu_seqlens_k, int64_t num_se
   if (reinterpret_cast<uint64_t>(plan) % 16 != 0) {
     return nkv_fail(NKV_E_INVALID, "nkv_build_shared_plan: plan must be 16-byte aligned");
   }
-  const GroupOf groups{cu_groups, prefix_lens, static_cast<int32_t>(num_groups), static_cast<int32_t>(num_seqs)};
+  const GroupOf groups{cu_seqlens_k, cu_groups, prefix_lens, static_cast<int32_t>(num_groups),
+                       static_cast<int32_t>(num_seqs)};
   const size_t lds = (static_cast<size_t>(std::max(num_seqs, num_groups)) + 1) * sizeof(int32_t);
   shared_plan_kernel<<<dim3(1), dim3(kPlanThreads), lds, static_cast<hipStream_t>(stream)>>>(
-      cu_seqlens_k, groups, static_cast<int32_t>(num_kv_heads), static_cast<int32_t>(group), shape,
-      static_cast<int4*>(plan));
+      groups, static_cast<int32_t>(num_kv_heads), static_cast<int32_t>(group), shape, static_cast<int4*>(plan));
   return nkv_check_launch("nkv_build_shared_plan");
 }
 

@@ -197,6 +197,16 @@ def test_sequences_shorter_than_the_prefix_are_read_alone(backend, gpu_device):
     assert bool(torch.isnan(bad[0]).all())
 
 
+@pytest.mark.parametrize("rests", [[-200, 5, 30], [-1, 17, 0, 64], [-60, 8, -3, 40]])
+def test_a_first_sequence_without_the_whole_prefix_shares_nothing(backend, gpu_device, rests):
+    """The prefix is read through the first sequence's table: where that has
+    not all of it (an empty row, a shorter context, its last blocks -1), the
+    others are read through their own."""
+    dev, host = make(gpu_device, [2, len(rests), 2], [70, 200, 90], [3, 9] + rests + [0, 11], seed=13)
+    dev["rest"] = -1
+    check(attend(backend, dev, 0.09), host, 0.09, rests)
+
+
 def test_rows_outside_the_contexts_do_not_matter(backend, gpu_device):
     """NaN and infinity in every row that no context holds."""
     dev, host = make(gpu_device, [5, 3], [37, 90], [3, 0, 17, 40, 1, 2, 80, 5], bs=32, seed=7)
