@@ -184,6 +184,7 @@ class DeviceBlockPool:
         self._args.append(0)
         moves = torch.empty((max(1, self.num_blocks // 2), 2), dtype=torch.int32, device=self.device)
         self._flush(moves)
+        self.copies = self.copies[:0]  # an earlier flush's: their ids have moved
         meta = self.meta.cpu().tolist()
         if meta[4]:
             raise RuntimeError(f"block pool op {int(meta[3]) - 1} failed: "
@@ -200,6 +201,7 @@ class DeviceBlockPool:
         the previous upload has completed.  `timer` (a
         nanokv.benchmark.LaunchTimer) brackets the apply kernel alone."""
         if not self._ops:
+            self.copies = self.copies[:0]  # the last log's are not copied twice
             return
         copies = torch.empty((self._pairs, 2), dtype=torch.int32, device=self.device)
         self._flush(copies, timer)

@@ -93,6 +93,40 @@ def test_copy_blocks_past_4_gib_and_refusals(backend, gpu_device):
             call()
 
 
+def test_copies_on_other_streams_and_in_graphs(backend, gpu_device):
+    """Pairs read at every replay: new ones, none (-1), ids that come and go."""
+    from nanokv.packing import capture_graph
+
+    gen = torch.Generator().manual_seed(3)
+    cache = torch.randn(2, 2, 12, 16, 2, 64, generator=gen).to(torch.bfloat16).to(gpu_device)
+    start = cache.clone()
+    pairs = torch.tensor([(0, 5), (0, 6), (1, 7)], dtype=torch.int32, device=gpu_device)
+
+    def copied(x, of):
+        x = x.clone()
+        for a, b in of:
+            if 0 <= a < 12 and 0 <= b < 12:
+                x[:, :, b] = x[:, :, a]
+        return x
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        backend.copy_blocks(cache, pairs)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(cache, copied(start, pairs.tolist()))
+    graph = torch.cuda.CUDAGraph()
+    with capture_graph(graph):
+        backend.copy_blocks(cache, pairs)
+    for of in ([(5, 0), (5, 1), (6, 2)], [(-1, -1)] * 3, [(3, 8), (12, 4), (8, -2)],
+               [(2, 9), (7, 10), (7, 11)]):
+        pairs.copy_(torch.tensor(of, dtype=torch.int32))
+        before = cache.clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(cache, copied(before, of)), of
+
+
 def test_forks_follow_the_oracle(gpu_device):
     """Random logs of allocations, appends, deallocations and forks, many
     forks in a row among them, forks of forks too."""
@@ -258,6 +292,24 @@ def test_compact_refuses_uncopied_forks(gpu_device):
         pool.compact()
     pool.flush()
     assert pool.compact().shape == (0, 2)
+
+
+def test_copies_are_one_logs_own(gpu_device):
+    """A step without calls, and a compaction, leave no pairs of an earlier
+    log to be copied again."""
+    pool = make_pool(gpu_device, 16, 4, 4, 4)
+    pool.allocate(0, 2)
+    pool.fork(0, 1, 6)
+    pool.flush()
+    assert pool.copies.shape == (1, 2)
+    pool.flush()
+    assert pool.copies.shape == (0, 2)
+    pool.fork(0, 2, 5)
+    pool.flush()
+    pool.deallocate(1)
+    assert pool.copies.shape == (1, 2)
+    pool.compact()
+    assert pool.copies.shape == (0, 2)
 
 
 def test_a_forked_sequence_goes_on_alone(backend, gpu_device):
