@@ -233,6 +233,43 @@ void (*rotary_kernel_for(bool interleaved, bool store))(RotaryArgs) {
   return store ? rotary_kernel<E, W, false, true> : rotary_kernel<E, W, false, false>;
 }
 
+// [tokens, heads, dim] elements of one tensor, addresses and strides in elements.
+struct HeadsView {
+  int64_t at, token, head, heads;
+};
+// The elements from the first to past the last of a token's heads, of all.
+int64_t span_of(const HeadsView& v, int64_t dim) { return (v.heads - 1) * v.head + dim; }
+int64_t extent_of(const HeadsView& v, int64_t tokens, int64_t dim) {
+  return (tokens - 1) * v.token + span_of(v, dim);
+}
+bool same_view(const HeadsView& a, const HeadsView& b, int64_t tokens) {
+  return a.at == b.at && a.heads == b.heads && (tokens == 1 || a.token == b.token) &&
+         (a.heads == 1 || a.head == b.head);
+}
+// Whether two elements of a view are one.
+bool folds(const HeadsView& v, int64_t tokens, int64_t dim) {
+  if (v.heads > 1 && v.head < dim) return true;
+  if (tokens > 1 && v.token < dim) return true;
+  return tokens > 1 && v.heads > 1 && v.token < span_of(v, dim) && v.head < (tokens - 1) * v.token + dim;
+}
+// Whether two views may have an element in common.  Views whose ranges meet
+// have none where they lie apart within one row or within one head's step of
+// the rows they are cut from (q, k and v of a fused projection).
+bool meet(const HeadsView& a, const HeadsView& b, int64_t tokens, int64_t dim) {
+  if (a.at + extent_of(a, tokens, dim) <= b.at || b.at + extent_of(b, tokens, dim) <= a.at) return false;
+  auto apart = [](int64_t step, int64_t delta, int64_t la, int64_t lb) {
+    const int64_t d = ((delta % step) + step) % step;
+    return d >= la && d + lb <= step;
+  };
+  if (tokens > 1 && a.token == b.token && a.token > 0 &&
+      apart(a.token, b.at - a.at, span_of(a, dim), span_of(b, dim))) {
+    return false;
+  }
+  return !(a.heads > 1 && b.heads > 1 && a.head == b.head && a.head > 0 &&
+           (tokens == 1 || (a.token % a.head == 0 && b.token % a.head == 0)) &&
+           apart(a.head, b.at - a.at, dim, dim));
+}
+
 }  // namespace
 }  // namespace nkv
 
@@ -315,6 +352,25 @@ extern "C" int nkv_rotary(const nkv_rotary_desc* d, void* stream) {
   if (bits % static_cast<uint64_t>(eb) != 0 || reinterpret_cast<uint64_t>(d->table) % 16 != 0 ||
       reinterpret_cast<uint64_t>(d->positions) % static_cast<uint64_t>(d->position_bytes) != 0) {
     return nkv_fail(NKV_E_INVALID, "nkv_rotary: pointers not aligned to their elements (table: 16 bytes)");
+  }
+  // Outputs: their own input or memory of their own, and no element twice.
+  auto view = [&](const void* p, int64_t token, int64_t head, int64_t n) {
+    return HeadsView{static_cast<int64_t>(reinterpret_cast<uint64_t>(p) / static_cast<uint64_t>(eb)), token, head, n};
+  };
+  const HeadsView q = view(d->q, d->q_token_stride, d->q_head_stride, d->num_q_heads);
+  const HeadsView k = view(d->k, d->k_token_stride, d->k_head_stride, d->num_kv_heads);
+  const HeadsView v = view(store ? d->v : nullptr, d->v_token_stride, d->v_head_stride, d->num_kv_heads);
+  const HeadsView qo = view(d->q_out, d->q_out_token_stride, d->q_out_head_stride, d->num_q_heads);
+  const HeadsView ko = view(d->k_out, d->k_out_token_stride, d->k_out_head_stride, d->num_kv_heads);
+  const bool has_q = d->num_q_heads > 0, has_k = d->num_kv_heads > 0, has_ko = has_k && d->k_out != nullptr;
+  const int64_t n = d->num_tokens, dim = d->head_dim;
+  if ((has_q && (folds(qo, n, dim) || (!same_view(qo, q, n) && meet(qo, q, n, dim)) ||
+                 (has_k && meet(qo, k, n, dim)) || (has_k && store && meet(qo, v, n, dim)))) ||
+      (has_ko && (folds(ko, n, dim) || (!same_view(ko, k, n) && meet(ko, k, n, dim)) ||
+                  (store && meet(ko, v, n, dim)) || (has_q && (meet(ko, q, n, dim) || meet(ko, qo, n, dim)))))) {
+    return nkv_fail(NKV_E_INVALID,
+                    "nkv_rotary: an output must be its own input or overlap no tensor of the call, "
+                    "and hold each element once");
   }
   uint64_t strides = 0;
   for (int64_t s : {d->q_token_stride, d->q_head_stride, d->k_token_stride, d->k_head_stride,

@@ -656,6 +656,9 @@ def _launch_rotary(q, k, v, key_cache, value_cache, slot_mapping, positions, tab
         _require_contiguous_cache("rotary store", key_cache, value_cache)
         slot_mapping = _int32_index("rotary store", "slot_mapping", slot_mapping)
         _require_store_rows(k, v, key_cache, value_cache, slot_mapping)
+        if key_cache.numel() == 0:  # no slot: k and v go nowhere
+            key_cache, k_out = None, torch.empty(k.shape, dtype=k.dtype, device=device) if k_out is None else k_out
+    if key_cache is not None:
         d.v, d.v_token_stride, d.v_head_stride = v.data_ptr(), v.stride(0), v.stride(1)
         d.key_cache, d.value_cache = key_cache.data_ptr(), value_cache.data_ptr()
         d.slot_mapping = slot_mapping.data_ptr()

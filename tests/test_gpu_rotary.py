@@ -197,6 +197,44 @@ def test_no_tokens_other_streams_and_graphs(backend, gpu_device):
         assert torch.equal(kc.view(64, 2, 128)[slots.long()], eager[1])
 
 
+@pytest.mark.parametrize("dim,interleaved", [(128, False), (128, True), (40, True)])
+@pytest.mark.parametrize("tokens", [1, 2, 33])
+def test_fused_projections_are_rotated_in_place(backend, gpu_device, dim, interleaved, tokens):
+    """q and k rotated where a projection left them, between its other parts:
+    a row's q, k and v one after another, or head by head."""
+    gen = torch.Generator().manual_seed(31)
+    table = RotaryTable(dim, 64, device=gpu_device)
+    fused = torch.randn(tokens, 3 * 4 * dim, generator=gen).to(torch.bfloat16).to(gpu_device)
+    if interleaved:
+        q, k, v = fused.view(tokens, 4, 3, dim).unbind(2)
+    else:
+        q, k, v = fused.view(tokens, 3, 4, dim).unbind(1)
+    positions = torch.randint(0, 64, (tokens,), generator=gen).to(gpu_device)
+    old_v = v.clone()
+    expected = backend.rotary(q, k, positions, table)
+    kc = torch.zeros(5, 16, 4, dim, dtype=torch.bfloat16, device=gpu_device)
+    vc = torch.zeros_like(kc)
+    slots = torch.arange(tokens, dtype=torch.int32, device=gpu_device)
+    out = backend.rotary_store(q, k, v, kc, vc, slots, positions, table, q_out=q, k_out=k)
+    assert out.data_ptr() == q.data_ptr()
+    assert torch.equal(q, expected[0]) and torch.equal(k, expected[1]) and torch.equal(v, old_v)
+    assert torch.equal(kc.view(-1, 4, dim)[:tokens], expected[1])
+    assert torch.equal(vc.view(-1, 4, dim)[:tokens], old_v)
+    with pytest.raises(RuntimeError, match="overlap"):
+        backend.rotary(q, k, positions, table, out=(k, torch.empty_like(k)))
+
+
+def test_a_cache_without_slots_stores_nothing(backend, gpu_device):
+    gen = torch.Generator().manual_seed(32)
+    table = RotaryTable(64, 32, device=gpu_device)
+    q, k, v = heads(gen, gpu_device, 5, torch.bfloat16, 2, 1, 64)
+    positions = torch.arange(5, device=gpu_device)
+    kc = torch.empty(0, 16, 1, 64, dtype=torch.bfloat16, device=gpu_device)
+    slots = torch.full((5,), -1, dtype=torch.int32, device=gpu_device)
+    out = backend.rotary_store(q, k, v, kc, torch.empty_like(kc), slots, positions, table)
+    assert torch.equal(out, backend.rotary(q, k, positions, table)[0])
+
+
 def test_rows_past_4_gib(backend, gpu_device):
     table = RotaryTable(128, 16, device=gpu_device)
     nb, bs = 8400, 256  # 2 KiB rows: 4.4 GB a cache

@@ -106,6 +106,26 @@ def test_bad_rotary_descriptors_fail_before_launch(changes, message):
     assert message in library.nkv_last_error().decode()
 
 
+BASE = dict(q=0x10000, k=0x20000, q_out=0x30000, k_out=0x40000, positions=0x50000, table=0x60000)
+
+
+@pytest.mark.parametrize("changes", [
+    dict(q_out=0x10000 + 16),                        # a shifted input
+    dict(q_out=0x10000, q_out_token_stride=64, q_out_head_stride=256),  # the input in another order
+    dict(q_out=0x20000), dict(k_out=0x10000), dict(k_out=0x30000 + 128),  # another tensor's memory
+    dict(q_out_token_stride=0), dict(q_out_head_stride=0), dict(q_out_head_stride=32),  # expanded
+    dict(q_out_token_stride=96), dict(k_out_token_stride=32),
+    dict(q=0x10000, k=0x10000 + 256, q_token_stride=192, k_token_stride=192, k_out=0x10000 + 128,
+         k_out_token_stride=192),                    # in a fused row, but q's second head
+    dict(k_out=0x20000, v=0x20000, v_token_stride=64, v_head_stride=64, key_cache=0x70000,
+         value_cache=0x80000, slot_mapping=0x90000, num_slots=4),  # k's output over v
+])
+def test_overlapping_rotary_outputs_fail_before_launch(changes):
+    library = _lib.load_library()
+    assert library.nkv_rotary(ctypes.byref(desc(**{**BASE, **changes})), None) != 0
+    assert "overlap" in library.nkv_last_error().decode()
+
+
 def test_other_bad_calls_fail_before_launch():
     lib = _lib.load_library()
     assert lib.nkv_rotary(None, None) != 0 and "null" in lib.nkv_last_error().decode()
@@ -118,6 +138,7 @@ def test_other_bad_calls_fail_before_launch():
             (lambda: lib.nkv_copy_blocks(64, 64, 1, 4, 4, 64, 4, 1, None), "8-byte"),
             (lambda: lib.nkv_copy_blocks(64, 64, 70000, 4, 4, 64, 64, 1, None), "too many"),
             (lambda: lib.nkv_copy_blocks(64, 64, 1, 4, 4, 8192, 64, 2**31, None), "too many"),
+            (lambda: lib.nkv_copy_blocks(64, 64, 1, 4, 4, 8192, 64, 2**24, None), "too many"),
             (lambda: lib.nkv_copy_blocks(65, 64, 1, 4, 4, 64, 64, 1, None), "aligned"),
             (lambda: lib.nkv_pool_apply_copies(None, None, 1, None, 0, None, 0, None), "null pool")):
         assert call() != 0
