@@ -65,7 +65,8 @@ extern "C" int nkv_copy_blocks(const void* src, void* dst, int64_t planes, int64
     return nkv_fail(NKV_E_INVALID, "nkv_copy_blocks: pairs must be 8-byte aligned");
   }
   const int64_t pieces = (block_bytes + kCopyBytes - 1) / kCopyBytes;
-  if (planes > 65535 || pieces > INT32_MAX || num_pairs > INT32_MAX / pieces) {
+  const int64_t most = UINT32_MAX / kCopyThreads;  // workgroups of a launch
+  if (planes > 65535 || pieces > most || num_pairs > most / pieces) {
     return nkv_fail(NKV_E_INVALID, "nkv_copy_blocks: too many pages or planes for one launch");
   }
   const int w = common_word_bytes({reinterpret_cast<uint64_t>(src), reinterpret_cast<uint64_t>(dst),

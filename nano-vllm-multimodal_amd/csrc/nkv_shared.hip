@@ -1207,7 +1207,9 @@ extern "C" int nkv_shared_prefix_attention_decode(
   }
   const int64_t items = shape.prefix * num_kv_heads + (shape.rest * num_kv_heads + 3) / 4;
   const int64_t pairs = num_seqs * num_q_heads;
-  if (items > INT32_MAX || pairs > INT32_MAX) {
+  const bool four = pairs <= kMergePairs;
+  const int64_t merges = four ? pairs : (pairs + 3) / 4;
+  if (items > UINT32_MAX / kThreads || merges > UINT32_MAX / kThreads) {
     return nkv_fail(NKV_E_INVALID, "%s: too many sequences and heads for one launch", what);
   }
   SharedArgs a;
@@ -1237,11 +1239,10 @@ extern "C" int nkv_shared_prefix_attention_decode(
               : (half ? shared_attention_kernel<false, true> : shared_attention_kernel<false, false>);
   kernel<<<dim3(static_cast<unsigned>(items)), dim3(kThreads), 0, s>>>(a);
   if (int rc = nkv_check_launch(what)) return rc;
-  const bool four = pairs <= kMergePairs;
   void (*merge)(SharedArgs, uint16_t*, int64_t) =
       four ? (half ? shared_merge_kernel<true, 4> : shared_merge_kernel<false, 4>)
            : (half ? shared_merge_kernel<true, 1> : shared_merge_kernel<false, 1>);
-  merge<<<dim3(static_cast<unsigned>(four ? pairs : (pairs + 3) / 4)), dim3(256), 0, s>>>(
+  merge<<<dim3(static_cast<unsigned>(merges)), dim3(256), 0, s>>>(
       a, static_cast<uint16_t*>(out), out_seq_stride);
   return nkv_check_launch(what);
 }

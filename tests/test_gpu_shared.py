@@ -318,6 +318,32 @@ def test_graph_replays_with_new_lengths_and_groups(backend, gpu_device):
         assert torch.equal(step(), out)
 
 
+def test_calls_on_two_streams_at_once(backend, gpu_device):
+    """Calls of different batches side by side, each with its workspace and
+    with an output inside a wider row."""
+    sets = []
+    for seed, sizes, prefixes in ((41, [9, 3], [400, 77]), (42, [1, 20], [50, 300])):
+        n = sum(sizes)
+        dev, host = make(gpu_device, sizes, prefixes, [(37 * i) % 150 for i in range(n)], kv=2, group=8,
+                         bs=16, seed=seed)
+        plan = backend.build_shared_prefix_plan(dev["kc"], dev["cu"], dev["total"], dev["groups"],
+                                                dev["prefix"], 16)
+        wide = torch.full((n, 18, 128), 5.0, dtype=torch.bfloat16, device=gpu_device)
+        sets.append((dev, host, plan, wide, torch.cuda.Stream()))
+    for *_, stream in sets:
+        stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for dev, _, plan, wide, stream in sets:
+            with torch.cuda.stream(stream):
+                attend(backend, dev, 0.1, plan=plan, out=wide[:, 1:17])
+    for *_, stream in sets:
+        torch.cuda.current_stream().wait_stream(stream)
+    for dev, host, plan, wide, _ in sets:
+        check(wide[:, 1:17], host, 0.1, "side by side")
+        assert torch.equal(wide[:, 1:17], attend(backend, dev, 0.1))
+        assert bool((wide[:, 0] == 5).all()) and bool((wide[:, 17] == 5).all())
+
+
 def test_caches_past_4_gib(backend, gpu_device):
     nb, bs = 8400, 256  # 2 KiB rows: 4.4 GB a cache
     kc = torch.zeros(nb, bs, 8, 128, dtype=torch.bfloat16, device=gpu_device)
