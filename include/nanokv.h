@@ -573,8 +573,12 @@ int nkv_transfer_synchronize(nkv_transfer* lane);
  *                number of moves goes to meta[5].
  *   Neither has a counterpart in the reference.  Both need
  *   nkv_pool_apply_copies, whose `copies` holds max_copies int32 pairs (those
- *   that no op writes become {-1, -1}); the pages themselves are moved by nkv_copy_blocks.  A FORK's pair is only
- *   good until a later op frees its source.
+ *   that no op writes become {-1, -1}); the pages themselves are moved by
+ *   nkv_copy_blocks.  A FORK's pair is only good until a later op frees its
+ *   source.
+ *   nkv_pool_apply_log is the same with the log in host memory, read before
+ *   the call returns: it goes with the launch, which bounds it to
+ *   NKV_POOL_LOG_WORDS words, 4 * num_ops + num_args (NKV_E_CAPACITY past it).
  *   Consecutive APPENDs, and consecutive ALLOCATEs without cached ids, run
  *   as one parallel step up to the first repeated slot; the result is the
  *   one-op-at-a-time result.
@@ -623,6 +627,7 @@ typedef struct nkv_pool_desc {
 #define NKV_POOL_ERR_BAD_ARGS 7      /* counts or args offset invalid    */
 #define NKV_POOL_MAX_BLOCKS (1 << 28)
 #define NKV_POOL_MAX_SEQS 65536
+#define NKV_POOL_LOG_WORDS 960
 int64_t nkv_pool_bytes(int64_t num_blocks, int64_t max_seqs,
                        int64_t max_blocks_per_seq);
 int nkv_pool_offsets(int64_t num_blocks, int64_t max_seqs,
@@ -633,6 +638,9 @@ int nkv_pool_apply(const nkv_pool_desc* pool, const int32_t* ops, int64_t num_op
 int nkv_pool_apply_copies(const nkv_pool_desc* pool, const int32_t* ops,
                           int64_t num_ops, const int32_t* args, int64_t num_args,
                           int32_t* copies, int64_t max_copies, void* stream);
+int nkv_pool_apply_log(const nkv_pool_desc* pool, const int32_t* ops,
+                       int64_t num_ops, const int32_t* args, int64_t num_args,
+                       int32_t* copies, int64_t max_copies, void* stream);
 int nkv_pack_decode_pool(const nkv_pool_desc* pool, const int32_t* num_tokens,
                          const int32_t* seq_slots, int64_t num_seqs,
                          int64_t padded_seqs, int64_t block_size,

@@ -39,6 +39,8 @@
 // bound by the latency of its loads and scans, one behind another: 63 forks of
 // 6 blocks 16 us (19 with each op read again instead of kept in LDS), a
 // compaction of 817 blocks and 96 tables 17, next to 69 and 420 us of pages.
+#include <cstring>
+
 #include "nkv_common.h"
 
 namespace nkv {
@@ -296,8 +298,8 @@ __device__ bool compact_blocks(const PoolView& v, Cursor& c, int2* __restrict__ 
 // ...] the ids (allocate); the parent slot, then the index of the pair to
 // write or -1 when the last block is shared too (fork); the index of the
 // first pair (compact).
-__global__ __launch_bounds__(kPoolThreads) void pool_apply_kernel(
-    PoolView v, const int4* __restrict__ ops, int64_t num_ops,
+__device__ __forceinline__ void pool_apply(
+    const PoolView& v, const int4* __restrict__ ops, int64_t num_ops,
     const int32_t* __restrict__ args, int64_t num_args, int2* __restrict__ copies,
     int64_t max_copies) {
   __shared__ int32_t s_tmp[kPoolThreads / kWave + 1];
@@ -747,6 +749,30 @@ __global__ __launch_bounds__(kPoolThreads) void pool_apply_kernel(
   }
 }
 
+__global__ __launch_bounds__(kPoolThreads) void pool_apply_kernel(
+    PoolView v, const int4* __restrict__ ops, int64_t num_ops,
+    const int32_t* __restrict__ args, int64_t num_args, int2* __restrict__ copies,
+    int64_t max_copies) {
+  pool_apply(v, ops, num_ops, args, num_args, copies, max_copies);
+}
+
+// A log that goes with the launch: no upload in front of it (3 us and its
+// place on the stream), and the ops, read one after another, come from LDS.
+struct PoolLog {
+  int4 words[NKV_POOL_LOG_WORDS / 4];
+};
+static_assert(sizeof(PoolLog) + sizeof(PoolView) + 32 <= 4096, "kernel arguments");
+__global__ __launch_bounds__(kPoolThreads) void pool_apply_log_kernel(
+    PoolView v, int32_t num_ops, int32_t num_args, int2* __restrict__ copies, int32_t max_copies,
+    PoolLog log) {
+  __shared__ int4 s_log[NKV_POOL_LOG_WORDS / 4];
+  const int32_t t = threadIdx.x;
+  if (t < NKV_POOL_LOG_WORDS / 4 && 4 * t < 4 * num_ops + num_args) s_log[t] = log.words[t];
+  __syncthreads();
+  pool_apply(v, s_log, num_ops, reinterpret_cast<const int32_t*>(s_log + num_ops), num_args, copies,
+             max_copies);
+}
+
 // Rejects descriptors the kernels could not use safely.
 int check_desc(const nkv_pool_desc* d, const char* what) {
   if (d == nullptr || d->memory == nullptr) return nkv_fail(NKV_E_INVALID, "%s: null pool", what);
@@ -792,15 +818,12 @@ extern "C" int nkv_pool_init(const nkv_pool_desc* pool, void* stream) {
   return nkv_check_launch("nkv_pool_init");
 }
 
-extern "C" int nkv_pool_apply(const nkv_pool_desc* pool, const int32_t* ops, int64_t num_ops,
-                              const int32_t* args, int64_t num_args, void* stream) {
-  return nkv_pool_apply_copies(pool, ops, num_ops, args, num_args, nullptr, 0, stream);
-}
+namespace nkv {
+namespace {
 
-extern "C" int nkv_pool_apply_copies(const nkv_pool_desc* pool, const int32_t* ops, int64_t num_ops,
-                                     const int32_t* args, int64_t num_args, int32_t* copies,
-                                     int64_t max_copies, void* stream) {
-  using namespace nkv;
+// The arguments that both forms of the call check alike.
+int check_log(const nkv_pool_desc* pool, const int32_t* ops, int64_t num_ops, const int32_t* args,
+              int64_t num_args, const int32_t* copies, int64_t max_copies) {
   if (int rc = check_desc(pool, "nkv_pool_apply")) return rc;
   if (max_copies < 0 || max_copies > INT32_MAX || (max_copies > 0 && copies == nullptr) ||
       reinterpret_cast<uint64_t>(copies) % 8 != 0) {
@@ -810,10 +833,26 @@ extern "C" int nkv_pool_apply_copies(const nkv_pool_desc* pool, const int32_t* o
   if (num_ops < 0 || num_args < 0 || num_ops > INT32_MAX || num_args > INT32_MAX) {
     return nkv_fail(NKV_E_INVALID, "nkv_pool_apply: negative or oversized op log");
   }
-  if (num_ops == 0) return NKV_OK;
-  if (ops == nullptr || (num_args > 0 && args == nullptr)) {
+  if (num_ops > 0 && (ops == nullptr || (num_args > 0 && args == nullptr))) {
     return nkv_fail(NKV_E_INVALID, "nkv_pool_apply: null pointer");
   }
+  return NKV_OK;
+}
+
+}  // namespace
+}  // namespace nkv
+
+extern "C" int nkv_pool_apply(const nkv_pool_desc* pool, const int32_t* ops, int64_t num_ops,
+                              const int32_t* args, int64_t num_args, void* stream) {
+  return nkv_pool_apply_copies(pool, ops, num_ops, args, num_args, nullptr, 0, stream);
+}
+
+extern "C" int nkv_pool_apply_copies(const nkv_pool_desc* pool, const int32_t* ops, int64_t num_ops,
+                                     const int32_t* args, int64_t num_args, int32_t* copies,
+                                     int64_t max_copies, void* stream) {
+  using namespace nkv;
+  if (int rc = check_log(pool, ops, num_ops, args, num_args, copies, max_copies)) return rc;
+  if (num_ops == 0) return NKV_OK;
   if (reinterpret_cast<uint64_t>(ops) % 16 != 0) {
     return nkv_fail(NKV_E_INVALID, "nkv_pool_apply: ops must be 16-byte aligned");
   }
@@ -821,6 +860,27 @@ extern "C" int nkv_pool_apply_copies(const nkv_pool_desc* pool, const int32_t* o
       view_of(*pool), reinterpret_cast<const int4*>(ops), num_ops, args, num_args,
       reinterpret_cast<int2*>(copies), max_copies);
   return nkv_check_launch("nkv_pool_apply");
+}
+
+extern "C" int nkv_pool_apply_log(const nkv_pool_desc* pool, const int32_t* ops, int64_t num_ops,
+                                  const int32_t* args, int64_t num_args, int32_t* copies,
+                                  int64_t max_copies, void* stream) {
+  using namespace nkv;
+  if (int rc = check_log(pool, ops, num_ops, args, num_args, copies, max_copies)) return rc;
+  if (4 * num_ops + num_args > NKV_POOL_LOG_WORDS) {
+    return nkv_fail(NKV_E_CAPACITY, "nkv_pool_apply_log: a log of %lld words, at most %d go with the launch",
+                    static_cast<long long>(4 * num_ops + num_args), NKV_POOL_LOG_WORDS);
+  }
+  if (num_ops == 0) return NKV_OK;
+  PoolLog log;
+  std::memcpy(log.words, ops, static_cast<size_t>(num_ops) * 16);
+  if (num_args > 0) {
+    std::memcpy(reinterpret_cast<int32_t*>(log.words) + 4 * num_ops, args, static_cast<size_t>(num_args) * 4);
+  }
+  pool_apply_log_kernel<<<dim3(1), dim3(kPoolThreads), 0, static_cast<hipStream_t>(stream)>>>(
+      view_of(*pool), static_cast<int32_t>(num_ops), static_cast<int32_t>(num_args),
+      reinterpret_cast<int2*>(copies), static_cast<int32_t>(max_copies), log);
+  return nkv_check_launch("nkv_pool_apply_log");
 }
 
 namespace nkv {

@@ -188,6 +188,8 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "nkv_pool_apply": (ctypes.c_int, (c_pool, c_ptr, c_i64, c_ptr, c_i64, c_ptr)),
     "nkv_pool_apply_copies": (
         ctypes.c_int, (c_pool, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr)),
+    "nkv_pool_apply_log": (
+        ctypes.c_int, (c_pool, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr)),
     "nkv_copy_blocks": (
         ctypes.c_int, (c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_ptr, c_i64, c_ptr)),
     "nkv_rotary_table": (ctypes.c_int, (c_ptr, ctypes.c_double, c_i64, c_i64, c_ptr, c_ptr)),
@@ -223,6 +225,7 @@ NKV_POOL_OP_APPEND = 3
 NKV_POOL_OP_FENCE = 4
 NKV_POOL_OP_FORK = 5
 NKV_POOL_OP_COMPACT = 6
+NKV_POOL_LOG_WORDS = 960
 NKV_POOL_ERRORS = {
     1: "unknown op type",
     2: "slot outside [0, max_seqs)",

@@ -294,6 +294,32 @@ def test_compact_refuses_uncopied_forks(gpu_device):
     assert pool.compact().shape == (0, 2)
 
 
+def test_logs_with_the_launch_and_uploaded_ones_agree(gpu_device, monkeypatch):
+    """The same logs at and around the length that the launch carries, and
+    with none of them short enough."""
+    from nanokv import _lib
+
+    def play(slots):
+        pool = make_pool(gpu_device, 3000, 16, 300, 8)
+        pool.allocate(0, 3)
+        for child in range(1, slots):
+            pool.fork(0, child, 40)  # 4 + 2 words each
+        pool.flush()
+        for child in range(2, slots, 3):
+            pool.deallocate(child)
+        for child in range(3, slots, 3):
+            pool.append(child)
+        moves = pool.compact()
+        return pool.snapshot(), pool.copies.tolist(), moves.tolist()
+
+    for slots in (2, 159, 160, 161, 300):
+        short = play(slots)
+        with monkeypatch.context() as patch:
+            patch.setattr(_lib, "NKV_POOL_LOG_WORDS", 0)
+            assert play(slots) == short, slots
+        assert short[0]["error"] is None
+
+
 def test_copies_are_one_logs_own(gpu_device):
     """A step without calls, and a compaction, leave no pairs of an earlier
     log to be copied again."""

@@ -140,6 +140,7 @@ def test_other_bad_calls_fail_before_launch():
             (lambda: lib.nkv_copy_blocks(64, 64, 1, 4, 4, 8192, 64, 2**31, None), "too many"),
             (lambda: lib.nkv_copy_blocks(64, 64, 1, 4, 4, 8192, 64, 2**24, None), "too many"),
             (lambda: lib.nkv_copy_blocks(65, 64, 1, 4, 4, 64, 64, 1, None), "aligned"),
+            (lambda: lib.nkv_pool_apply_log(None, None, 1, None, 0, None, 0, None), "null pool"),
             (lambda: lib.nkv_pool_apply_copies(None, None, 1, None, 0, None, 0, None), "null pool")):
         assert call() != 0
         assert message in lib.nkv_last_error().decode(), message
