@@ -9,6 +9,10 @@ Layout:
                     registration
   nanokv.packing    device-side packing of cu_seqlens / slot_mapping /
                     block_tables from per-sequence scheduler state
+  nanokv.pool       block bookkeeping on the device: allocate, append, fork,
+                    compact
+  nanokv.rotary     tables of rotary positions for ``backend.rotary`` and
+                    ``backend.rotary_store``
   nanokv.workloads  seeded synthetic workloads (decode store, chunked
                     prefill, prefix-cache gather, narrow rows, decode step)
   nanokv.benchmark  timing, byte accounting and percentiles
