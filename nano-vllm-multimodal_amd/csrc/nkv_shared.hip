@@ -71,8 +71,13 @@ constexpr int kMinRestChunks = 4;
 // cut for two 32.0; up to 12 and 16 tiles the same).  8 sequences behind
 // 1,511 keys take 12.6 us from 1 or 2 tiles on, 14.5 from 4.  Longer ones pay
 // for the second workgroup: it takes its weights while the first multiplies
-// (16,384 keys alone 60 us, cut for one 71).
+// (16,384 keys alone 60 us, cut for one 71).  Beside long rests, more than
+// kRestsPerTile chunks per tile, the rests take that second place, and a cut
+// for one leaves no CU with two pieces while others have one (256 sequences of
+// 32 heads behind 4,096 keys, 16 to 256 of their own: 50 us instead of 56;
+// 1,024 of them 160 instead of 175; at 1.5 chunks per tile 45.3 instead of 43.6).
 constexpr int kMinPieceTiles = 2;
+constexpr int kRestsPerTile = 2;
 constexpr int kWidePieceTiles = 8;
 constexpr int32_t kMaxLength = 0x7FFFFF00;
 constexpr float kRescaleLog2 = 8.f;  // the reference max moves only past this
@@ -206,8 +211,9 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
   const int64_t slots = slots_per_head(num_kv_heads);
   const int64_t share = (prefix_units + rest_units / 4 + slots - 1) / slots;
   const int64_t half = (2 * prefix_units + slots - 1) / slots;  // a workgroup per CU
+  const bool wide = rest_units > kRestsPerTile * prefix_units;
   const int64_t prefix_tiles = max(max(static_cast<int64_t>(kMinPieceTiles), share),
-                                   min(half, static_cast<int64_t>(kWidePieceTiles)));
+                                   wide ? half : min(half, static_cast<int64_t>(kWidePieceTiles)));
   const int64_t room = max(static_cast<int64_t>(1), shape.rest - num_seqs);
   const int64_t rest_chunks =
       max(max(static_cast<int64_t>(kMinRestChunks), rest_units / (4 * slots * kRestRounds) + 1),
