@@ -666,7 +666,10 @@ def validate_groups(cu_seqlens_k: torch.Tensor, cu_groups: torch.Tensor, prefix_
 
 
 def validate_positions(positions: torch.Tensor, table) -> None:
-    """Position values, when index validation is enabled (it synchronises)."""
+    """The rows that the table takes; position values, when index validation
+    is enabled (it synchronises)."""
+    if positions.ndim == 2 and table.sections is None:
+        raise ValueError("three position rows need a rotary table with sections")
     if positions.numel() and index_value_validation_enabled(positions):
         if bool(((positions < 0) | (positions >= table.max_position)).any()):
             raise ValueError(f"positions contain one outside [0, {table.max_position})")

@@ -645,8 +645,6 @@ def _launch_rotary(q, k, v, key_cache, value_cache, slot_mapping, positions, tab
         raise ValueError("section_ends must hold two counts of pairs")
     row_stride = 0
     if positions.ndim == 2:
-        if ends == (half, half):
-            raise ValueError("three position rows need a rotary table with sections")
         if positions.stride(0) < tokens:  # an expanded row: three rows of their own
             positions = positions.contiguous()
         row_stride = positions.stride(0)

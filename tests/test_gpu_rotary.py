@@ -224,6 +224,16 @@ def test_fused_projections_are_rotated_in_place(backend, gpu_device, dim, interl
         backend.rotary(q, k, positions, table, out=(k, torch.empty_like(k)))
 
 
+@pytest.mark.parametrize("sections", [(32, 0, 0), (0, 32, 0), (0, 0, 32)])
+def test_one_row_of_three_positions_may_turn_every_pair(backend, gpu_device, sections):
+    gen = torch.Generator().manual_seed(33)
+    q, k, v = heads(gen, gpu_device, 9, torch.bfloat16, 2, 1, 64)
+    positions = torch.randint(0, 50, (3, 9), generator=gen).to(gpu_device)
+    got = backend.rotary(q, k, positions, RotaryTable(64, 50, sections=sections, device=gpu_device))
+    plain = backend.rotary(q, k, positions[sections.index(32)].contiguous(), RotaryTable(64, 50, device=gpu_device))
+    assert torch.equal(got[0], plain[0]) and torch.equal(got[1], plain[1])
+
+
 def test_a_cache_without_slots_stores_nothing(backend, gpu_device):
     gen = torch.Generator().manual_seed(32)
     table = RotaryTable(64, 32, device=gpu_device)
