@@ -489,7 +489,8 @@ __device__ __forceinline__ void attend(TileShared& sh, const KeySource& src, con
     }
     return tile;
   };
-  // (A group of up to 64 rows is one tile: nothing else reads its keys.)
+  // (Up to 64 rows are a whole group, whose keys nothing else reads, or the
+  // last of its tiles, behind those that keep them in the caches.)
   const ChunkCopy<kChunked, RW != 4> copy(src, lane);
   const uint32_t lds_k = lds_address(&sh.k[0][0]) + chunk * 4096u;
   const uint32_t lds_v = lds_address(&sh.v[0][0]) + chunk * 4096u;

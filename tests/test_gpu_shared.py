@@ -399,6 +399,37 @@ def test_fork_rotate_store_and_attend_together(backend, gpu_device):
     assert torch.equal(cache[0, 0].view(-1, kv, 128)[slots.long()], backend.rotary(q, k, positions, table)[1])
 
 
+def test_the_registered_ops_are_the_backends(backend, gpu_device):
+    """torch.ops by their schemas, as a caller of the other ops finds them."""
+    from nanokv.rotary import RotaryTable
+
+    ops = torch.ops.nanovllm_paged_kv
+    dev, _ = make(gpu_device, [5, 3], [130, 40], [7, 0, 33, 1, 90, 5, 5, 64], kv=2, group=4, seed=23)
+    expected = attend(backend, dev, 0.1)
+    plan = ops.build_shared_prefix_plan(dev["cu"], dev["groups"], dev["prefix"], 2, 8, -1)
+    out = torch.empty_like(expected)
+    ops.shared_prefix_attention_decode(dev["q"], dev["kc"], dev["vc"], dev["tables"], plan, 2, -1, 0.1, out)
+    other = backend.build_shared_prefix_plan(dev["kc"], dev["cu"], dev["total"], dev["groups"], dev["prefix"], 8)
+    other.plan, other.rest_tokens = plan, -1
+    assert torch.equal(out, attend(backend, dev, 0.1, plan=other))
+    table = RotaryTable(128, 300, device=gpu_device)
+    positions = torch.arange(8, device=gpu_device) * 30
+    q, k = dev["q"], torch.randn(8, 2, 128, device=gpu_device).to(torch.bfloat16)
+    ref = backend.rotary(q, k, positions, table)
+    q_out, k_out = torch.empty_like(ref[0]), torch.empty_like(ref[1])
+    ops.rotary(q, k, positions, table.table, 0, [64, 64], q_out, k_out)
+    assert torch.equal(q_out, ref[0]) and torch.equal(k_out, ref[1])
+    kc, vc = dev["kc"].clone(), dev["vc"].clone()
+    slots = torch.tensor([3, 5, -1, 7, 40, 41, 42, 43], dtype=torch.int32, device=gpu_device)
+    ops.rotary_store(q, k, k, kc, vc, slots, positions, table.table, 0, [64, 64], q_out)
+    backend.store(ref[1], k, dev["kc"], dev["vc"], slots)
+    assert torch.equal(kc, dev["kc"]) and torch.equal(vc, dev["vc"]) and torch.equal(q_out, ref[0])
+    pairs = torch.tensor([[0, 3], [1, 4]], dtype=torch.int32, device=gpu_device)
+    ops.copy_blocks(kc, kc, pairs)
+    backend.copy_blocks(dev["kc"], pairs)
+    assert torch.equal(kc, dev["kc"]) and torch.equal(kc[3], kc[0])
+
+
 def test_refusals(backend, gpu_device, monkeypatch):
     dev, _ = make(gpu_device, [4, 2], [33, 20], [5] * 6, seed=19)
     plan = backend.build_shared_prefix_plan(dev["kc"], dev["cu"], dev["total"], dev["groups"],
