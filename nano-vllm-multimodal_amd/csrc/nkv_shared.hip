@@ -35,7 +35,7 @@
 // a row of zeros and their scores become -inf.
 //
 // 256 sequences of 16 query and 8 kv heads behind 16,384 shared keys, 16 to
-// 2,048 of their own (bf16, 533 MB, 35 GFLOP): 120 us; the rests alone 94 us,
+// 2,048 of their own (bf16, 533 MB, 35 GFLOP): 114 us; the rests alone 94 us,
 // 5.0 TB/s, the prefix alone 60 us.  Reading the prefix once per sequence
 // instead is 17.7 GB.  32 sequences of 28 and 4 heads behind 12,001 keys: 27
 // us, of which 21 are the attention; 8 sequences, 12 us, two launches' latency.
@@ -93,7 +93,7 @@ typedef __attribute__((address_space(4))) const int32_t const_i32;
 //   [2, 18)  256 bytes of zeros, the row that dropped keys copy
 //   two per sequence  {rest's first row, context length, first rest entry, rest entries}
 //                     {first entry of its group's first tile, pieces per tile, member, 0}
-//   two per prefix entry  {first sequence, first query row, query rows, 0}
+//   two per prefix entry  {first sequence, first query row, query rows, piece}
 //                         {first key, past the last, 0, 0}
 //   one per rest entry  {sequence, first row, past the last, 0}
 // Entries past the last of their kind are empty, so that a workgroup finds
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan_kernel(
     const int32_t key_tiles = (rows - 1) / kTileKeys + 1;
     const int32_t k0 = static_cast<int32_t>(static_cast<int64_t>(key_tiles) * piece / pieces) * kTileKeys;
     const int32_t k1 = min(rows, static_cast<int32_t>(static_cast<int64_t>(key_tiles) * (piece + 1) / pieces) * kTileKeys);
-    plan[shape.prefix_at() + 2 * e] = make_int4(first, tile * kTileRows, tile_q, 0);
+    plan[shape.prefix_at() + 2 * e] = make_int4(first, tile * kTileRows, tile_q, piece);
     plan[shape.prefix_at() + 2 * e + 1] = make_int4(k0, k1, 0, 0);
   }
   for (int32_t e = prefix_entries + t; e < shape.prefix; e += kPlanThreads) {
@@ -940,7 +940,10 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   const bool fits = plan_fits(plan, a.num_seqs, a.num_groups, a.num_kv_heads, a.group);
   // Workgroups of the prefix's entries, one per kv head each; then one per
   // four (rest entry, kv head) items.  The kv head rotates with the entry, so
-  // that no XCD (workgroup id % 8) stays on one byte offset of the rows.
+  // that no XCD (workgroup id % 8) stays on one byte offset of the rows; with
+  // the piece of a prefix, so that the tiles that read the same keys, a whole
+  // number of 8 workgroups apart from 8 kv heads on, share an L2 (256 sequences
+  // of 16 heads behind 16,384 keys 121.2 us; turned with the entry 124.2).
   const int64_t prefix_groups = a.shape.prefix * a.num_kv_heads;
   const bool is_prefix = blockIdx.x < prefix_groups;
   int64_t item = blockIdx.x;
@@ -949,8 +952,9 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   }
   const int32_t entry = static_cast<int32_t>(item / a.num_kv_heads);
   const int32_t turn = static_cast<int32_t>(item - static_cast<int64_t>(entry) * a.num_kv_heads);
-  const int32_t period = 8 / min(8, a.num_kv_heads & -a.num_kv_heads);
-  const int32_t kh = (turn + (is_prefix ? entry / period : 4 * (entry & 0xFFFF))) % a.num_kv_heads;
+  const const_i32* const prefix_record = plan + 4 * (a.shape.prefix_at() + 2 * static_cast<int64_t>(entry));
+  const int32_t turned = is_prefix ? max(0, prefix_record[3]) : 4 * (entry & 0xFFFF);
+  const int32_t kh = static_cast<int32_t>((static_cast<uint32_t>(turn) + turned) % a.num_kv_heads);
   KeySource src;
   src.k_head = a.key_cache + static_cast<int64_t>(kh) * (kDim * 2);
   src.v_head = a.value_cache + static_cast<int64_t>(kh) * (kDim * 2);
@@ -965,7 +969,7 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedArg
   rows.seq_stride = a.q_seq_stride;
   rows.group = a.group;
   if (is_prefix) {
-    const const_i32* const e = plan + 4 * (a.shape.prefix_at() + 2 * entry);
+    const const_i32* const e = prefix_record;
     rows.first = e[0];
     rows.row0 = e[1];
     rows.rows = e[2];
